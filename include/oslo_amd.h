@@ -575,6 +575,174 @@ int oslo_attention_prefill_bwd_stored(void *dq, void *dk, void *dv,
                                       const int64_t *strides, int dtype,
                                       oslo_stream_t stream);
 
+/* Sequences of different lengths ---------------------------------------------- */
+
+/*
+ * Causal attention over sequences laid one behind the other along one row of
+ * `tokens` tokens; query heads share key/value heads in groups of
+ * heads / kv_heads (head h reads key/value head h / group):
+ *   out[i, h, :] = sum over the tokens j <= i of i's own sequence of
+ *                  softmax_j(scale * q[i, h, :] . k[j, h / group, :]) * v[j, h / group, :]
+ * window > 0: only j > i - window. q, out: 16-bit, `tokens` x heads x head_dim
+ * (64, 128 or 256); k, v with kv_heads; strides[8] = the head and token strides,
+ * in elements, of q, k, v and out (multiples of 8, features contiguous, pointers
+ * 16-byte aligned, a sequence of a head under 2 GiB).
+ * blocks: int32 [num_blocks][4] in device memory, one entry (start, length, b,
+ * unused) for the b-th 128 tokens of the sequence of `length` tokens that begins
+ * at token `start`; every sequence needs ceil(length / 128) entries, in any
+ * order (most keys first runs fastest). max_length: no length exceeds it.
+ * Entries that do not describe tokens of the row or exceed max_length are passed
+ * over. Tokens of no sequence are neither read nor written.
+ * lse: NULL, or fp32 [heads, tokens], 16-byte aligned: log2 of the row's sum of
+ * 2^(log2(e) * scale * q.k), which the backward takes. Rounding as in
+ * oslo_attention_prefill_fwd. scale > 0. No workspace.
+ * No counterpart in the reference, whose attention takes padded batches
+ * (oslo/models/gptj/modeling_gptj.py:936-951).
+ */
+int oslo_attention_packed_fwd(void *out, float *lse, const void *q,
+                              const void *k, const void *v,
+                              const int32_t *blocks, int64_t num_blocks,
+                              float scale, int64_t tokens, int64_t max_length,
+                              int64_t heads, int64_t kv_heads,
+                              int64_t head_dim, int64_t window,
+                              const int64_t *strides, int dtype,
+                              oslo_stream_t stream);
+
+/* Bytes of fp32 workspace oslo_attention_packed_bwd needs. */
+size_t oslo_attention_packed_bwd_workspace_bytes(int64_t tokens, int64_t heads);
+
+/*
+ * Gradients of the packed attention from dout, the inputs, the forward's out and
+ * lse: the formulas of oslo_attention_prefill_bwd per sequence; dk and dv are
+ * summed over the query heads of a group in fp32, in a fixed order, and rounded
+ * once. query_blocks and key_blocks hold the same entries as the forward's
+ * `blocks` (most keys first, and most queries left first, run fastest).
+ * strides[16]: head and token strides of q, k, v, out, dout, dq, dk, dv. Rows of
+ * no sequence are not written. workspace: 16-byte aligned, contents irrelevant
+ * before and after. No output may alias an input. Same bits from run to run.
+ * No counterpart in the reference (see above).
+ */
+int oslo_attention_packed_bwd(void *dq, void *dk, void *dv, const void *dout,
+                              const void *q, const void *k, const void *v,
+                              const void *out, const float *lse,
+                              float *workspace, const int32_t *query_blocks,
+                              const int32_t *key_blocks, int64_t num_blocks,
+                              float scale, int64_t tokens, int64_t max_length,
+                              int64_t heads, int64_t kv_heads,
+                              int64_t head_dim, int64_t window,
+                              const int64_t *strides, int dtype,
+                              oslo_stream_t stream);
+
+/*
+ * The paged key/value cache. key_pages, value_pages: [num_pages, kv_heads,
+ * page_size, head_dim], page_size a power of two from 16 to 4096, head_dim 64,
+ * 128 or 256, 16-byte aligned. table: int32 [sequences, max_pages], the page that
+ * holds positions [i * page_size, (i + 1) * page_size) of each sequence. With
+ * key_scales and value_scales NULL the pages are of `dtype` (fp16 or bf16).
+ * With both given (uint8 [num_pages, kv_heads, page_size], 16-byte aligned)
+ * they are OCP e4m3: a vector x of head_dim features is kept as
+ * q = round_to_nearest_even_e4m3(x * 2^-e) and the byte e + 127, e the least
+ * integer >= -126 with max|x| <= 448 * 2^e over the finite features (0 if they
+ * are all 0); infinities and NaN are kept as NaN.
+ *
+ * write: token t of key, value ([tokens, kv_heads, head_dim] of `dtype`;
+ * strides[4] = head and token strides of key, then of value, in elements,
+ * multiples of 8) goes to position[t] of sequence[t]. Tokens whose sequence is
+ * outside the table, whose position is negative or beyond max_pages pages, or
+ * whose page number is outside the pool are passed over. Two tokens of one call
+ * must not name the same place. read: the same tokens out of the cache, as dense
+ * [tokens, kv_heads, head_dim] of `dtype` (8-bit values times their scale,
+ * rounded once where `dtype` cannot hold the product); tokens passed over by the
+ * write read as zeros.
+ * No counterpart in the reference, whose cache grows by concatenation
+ * (oslo/models/gptj/modeling_gptj.py:205-233).
+ */
+int oslo_paged_kv_write(void *key_pages, void *value_pages, uint8_t *key_scales,
+                        uint8_t *value_scales, const void *key,
+                        const void *value, const int32_t *sequence,
+                        const int32_t *position, const int32_t *table,
+                        int64_t tokens, int64_t sequences, int64_t max_pages,
+                        int64_t num_pages, int64_t kv_heads, int64_t page_size,
+                        int64_t head_dim, const int64_t *strides, int dtype,
+                        oslo_stream_t stream);
+int oslo_paged_kv_read(void *key, void *value, const void *key_pages,
+                       const void *value_pages, const uint8_t *key_scales,
+                       const uint8_t *value_scales, const int32_t *sequence,
+                       const int32_t *position, const int32_t *table,
+                       int64_t tokens, int64_t sequences, int64_t max_pages,
+                       int64_t num_pages, int64_t kv_heads, int64_t page_size,
+                       int64_t head_dim, int dtype, oslo_stream_t stream);
+
+/* Bytes of fp32 workspace oslo_attention_paged_decode_fwd needs (0: none);
+ * max_length = max_pages * page_size. */
+size_t oslo_attention_paged_decode_workspace_bytes(int64_t sequences,
+                                                   int64_t heads,
+                                                   int64_t kv_heads,
+                                                   int64_t head_dim,
+                                                   int64_t max_length,
+                                                   int64_t window);
+
+/*
+ * Attention of one new token per sequence over the paged cache:
+ *   out[b, h, :] = sum_p softmax_p(scale * q[b, h, :] . k[p, h / group, :]) * v[p, h / group, :]
+ * over the positions p < lengths[b] of sequence b (window > 0: the last `window`
+ * of them). q: [sequences, heads, head_dim] of `dtype`, strides[2] = its sequence
+ * and head strides in elements (multiples of 8); out dense. lengths: int32
+ * [sequences] in device memory, read by the kernel: a captured call may be
+ * replayed while they grow. A sequence of length 0 (or less) gives zeros; one that
+ * is longer than its table, or that would read a page number outside the pool,
+ * gives NaN and reads nothing out of bounds. Positions outside the visible ones
+ * are not looked at, whatever they hold. Products are of 16-bit values (an 8-bit
+ * cache's are exact in either type), sums and the softmax fp32, probabilities
+ * rounded to 16 bits before they multiply v, the result rounded once. The joining
+ * order is fixed: same bits from run to run. workspace:
+ * oslo_attention_paged_decode_workspace_bytes bytes, 16-byte aligned, contents
+ * irrelevant before and after; calls that may run at the same time need one each.
+ * No counterpart in the reference (its decoding attends a dense cache,
+ * oslo/models/gptj/modeling_gptj.py:936-951).
+ */
+int oslo_attention_paged_decode_fwd(void *out, const void *q,
+                                    const void *key_pages,
+                                    const void *value_pages,
+                                    const uint8_t *key_scales,
+                                    const uint8_t *value_scales,
+                                    const int32_t *table,
+                                    const int32_t *lengths, float *workspace,
+                                    float scale, int64_t sequences,
+                                    int64_t max_pages, int64_t num_pages,
+                                    int64_t heads, int64_t kv_heads,
+                                    int64_t page_size, int64_t head_dim,
+                                    int64_t window, const int64_t *strides,
+                                    int dtype, oslo_stream_t stream);
+
+/* Sampling ---------------------------------------------------------------------- */
+
+/*
+ * Draws one token per row of logits ([rows, vocab] of any dtype, row_stride
+ * elements apart) from uniforms[rows] in [0, 1). With x = logit / temperature and
+ * mass(j) = exp(x_j - max x), "before" meaning larger logit first and lower index
+ * first among equals: the first top_k tokens stay (0 or less: all); of those the
+ * shortest front with mass >= top_p times theirs (1 or more: all; at least one
+ * token); of those the ones with mass >= min_p. tokens[r] (int64) is the first
+ * index, in index order, at which the running mass of what stayed exceeds
+ * uniforms[r] times all of it; logprobs[r] (fp32, or NULL) the logarithm of its
+ * share. A temperature that is not positive takes the largest logit (lowest index
+ * first). NaN counts as -inf; -inf is never drawn; a row of nothing else gives
+ * token -1 and -inf. Uniforms outside [0, 1) are taken to its nearest end.
+ * Every setting is a number of the call or, where the pointer is given, one per
+ * row (fp32, top_k int32). Masses are summed as whole multiples of
+ * 2^(ceil(log2 vocab) - 62) of the largest: the token does not depend on the order of
+ * a sum. vocab up to 2^24. No workspace.
+ * The reference samples on the framework's operators after sorting
+ * (oslo/generation_utils.py).
+ */
+int oslo_sample(int64_t *tokens, float *logprobs, const void *logits,
+                const float *uniforms, const float *temperatures,
+                double temperature, const int32_t *top_ks, int64_t top_k,
+                const float *top_ps, double top_p, const float *min_ps,
+                double min_p, int64_t rows, int64_t vocab, int64_t row_stride,
+                int dtype, oslo_stream_t stream);
+
 /* Repeated n-gram blocking (beam search) ------------------------------------ */
 
 /*

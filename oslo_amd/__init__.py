@@ -15,7 +15,11 @@ from .fused_kernels_utils import (  # noqa: F401
     FusedLinearRows,
     FusedMergeHeads,
     FusedNoRepeatNGramLogitsProcessor,
+    FusedPackedAttention,
+    FusedPagedDecodeAttention,
+    FusedPagedKV,
     FusedRotaryPositionEmbedding,
+    FusedSampling,
     FusedScaleMaskSoftmax,
     FusedSplitHeads,
     FusedScaleMaskSoftmaxDropout,
@@ -30,5 +34,6 @@ from .modeling_gpt2 import GPT2Config, GPT2LMHeadModel  # noqa: F401
 from .modeling_gpt_neo import GPTNeoConfig, GPTNeoForCausalLM  # noqa: F401
 from .modeling_gptj import GPTJConfig, GPTJForCausalLM  # noqa: F401
 from .modeling_utils import DecodeState, StaticKV  # noqa: F401
+from .sequences import PackedSequences, PagedKV  # noqa: F401
 
 __version__ = "0.1.0"

@@ -78,6 +78,20 @@ PROTOTYPES = {
     "oslo_attention_prefill_bwd_stored": (
         _c.c_int, [_P] * 11 + [_c.c_size_t, _P, _c.c_float, _c.c_float, _U64, _U64, _I64, _I64, _I64, _I64, _I64,
                                _c.POINTER(_c.c_int64), _c.c_int, _P]),
+    "oslo_attention_packed_fwd": (
+        _c.c_int, [_P] * 6 + [_I64, _c.c_float] + [_I64] * 6 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
+    "oslo_attention_packed_bwd_workspace_bytes": (_c.c_size_t, [_I64, _I64]),
+    "oslo_attention_packed_bwd": (
+        _c.c_int, [_P] * 12 + [_I64, _c.c_float] + [_I64] * 6 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
+    "oslo_paged_kv_write": (
+        _c.c_int, [_P] * 9 + [_I64] * 7 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
+    "oslo_paged_kv_read": (_c.c_int, [_P] * 9 + [_I64] * 7 + [_c.c_int, _P]),
+    "oslo_attention_paged_decode_workspace_bytes": (_c.c_size_t, [_I64] * 6),
+    "oslo_attention_paged_decode_fwd": (
+        _c.c_int, [_P] * 9 + [_c.c_float] + [_I64] * 8 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
+    "oslo_sample": (
+        _c.c_int, [_P, _P, _P, _P, _P, _c.c_double, _P, _I64, _P, _c.c_double, _P, _c.c_double, _I64, _I64, _I64,
+                   _c.c_int, _P]),
     "oslo_ngram_repeat_block": (
         _c.c_int, [_P, _P, _I64, _I64, _I64, _I64, _c.c_int, _P]),
     "oslo_sample_idx_rows": (_I64, [_c.c_int32, _c.c_int32, _I64]),

@@ -41,6 +41,11 @@ SOURCES = [
     "attention_decode.hip",
     "attention_prefill.hip",
     "attention_prefill_bwd.hip",
+    "attention_packed.hip",
+    "attention_packed_bwd.hip",
+    "paged_kv.hip",
+    "attention_paged_decode.hip",
+    "sampling.hip",
     "dataset_index.hip",
 ]
 
@@ -62,14 +67,16 @@ FLAGS = [
 ]
 
 
-# The two prompt-attention sources name M0 as clobbered by their hand-written
+# The prompt-attention sources name M0 as clobbered by their hand-written
 # loads into LDS (they set it themselves inside the asm statement). M0 is a
 # reserved register to the compiler, which says so once per instantiation of
-# every such statement, thousands of lines per build; silenced for these two
+# every such statement, thousands of lines per build; silenced for these
 # files only, so that -Wall stays readable for everything else.
 EXTRA_FLAGS = {
     "attention_prefill.hip": ["-Wno-inline-asm"],
     "attention_prefill_bwd.hip": ["-Wno-inline-asm"],
+    "attention_packed.hip": ["-Wno-inline-asm"],
+    "attention_packed_bwd.hip": ["-Wno-inline-asm"],
 }
 if os.environ.get("OSLO_STORED_BUFFERS"):
     EXTRA_FLAGS["attention_prefill_bwd.hip"].append("-DOSLO_STORED_BUFFERS=" + str(int(os.environ["OSLO_STORED_BUFFERS"])))

@@ -134,6 +134,44 @@ __device__ __forceinline__ void wait_vm() {
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
 
+// Sequences of different lengths laid one behind the other along one row of
+// `tokens` tokens. The work is listed: an entry is a run of positions
+// (`block`-th of the sequence) of the sequence of `length` tokens that begins at
+// token `start`; empty sequences have none. Blocks of the grid go through the
+// heads first: consecutive blocks take consecutive entries of heads, and the
+// hardware hands consecutive blocks to consecutive XCDs, so the blocks of a key/value
+// head land on few of them (on one where the head count is a multiple of 8) and
+// its keys and values are read into few L2 caches. The heads of a group share
+// their keys, so neighbouring blocks take heads of different groups.
+struct PackedBlock {
+  int64_t start;
+  int length, block;
+};
+struct PackedArgs {
+  const int *blocks; // [number of blocks][4]: start, length, block, unused
+  int64_t tokens;    // of the whole row
+  int max_length;    // no sequence is longer (what the 32-bit offsets were checked against)
+  int kv_heads, group;
+};
+__device__ __forceinline__ PackedBlock packed_block(const PackedArgs &a, unsigned index) {
+  const int *e = a.blocks + 4 * (int64_t)index;
+  PackedBlock p;
+  p.start = __builtin_amdgcn_readfirstlane(e[0]);
+  p.length = __builtin_amdgcn_readfirstlane(e[1]);
+  p.block = __builtin_amdgcn_readfirstlane(e[2]);
+  return p;
+}
+// The list lies in device memory, where the host cannot check it: an entry that
+// does not describe positions of the row is passed over.
+__device__ __forceinline__ bool packed_block_in_range(const PackedArgs &a, const PackedBlock &e, int positions) {
+  return e.start >= 0 && e.length > 0 && e.length <= a.max_length && e.start + e.length <= a.tokens && e.block >= 0 &&
+         (int64_t)e.block * positions < e.length;
+}
+// The query head of the r-th block of an entry (r below the number of query heads).
+__device__ __forceinline__ int packed_query_head(const PackedArgs &a, int r) {
+  return (r % a.kv_heads) * a.group + r / a.kv_heads;
+}
+
 // Additive mask values below kMaskFloor act as kMaskFloor, in the forward and in
 // every pass of the backward (one constant, applied to the value in natural
 // units before anything else). Callers build masks of -10000, of -inf or of the

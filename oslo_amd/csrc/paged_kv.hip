@@ -1,0 +1,218 @@
+// Keys and values of new tokens into the paged cache, and back out of it: one
+// pass over the tokens' vectors each way, in 16 bits (a copy) or 8 bits
+// (e4m3 with a power-of-two scale per token and head, paged.hpp):
+//   write: e = least integer with max|x| <= 448 * 2^e;  q = round_to_e4m3(x * 2^-e)
+//   read:  x = q * 2^e
+// The vector of one token and head is held by D / 8 lanes, 16 bytes each, so
+// its largest magnitude is a reduction inside those lanes and it is read once.
+// Bound by HBM.
+
+#include "paged.hpp"
+
+namespace oslo {
+namespace {
+
+struct PagedKVArgs {
+  void *key_pages, *value_pages;
+  unsigned char *key_scales, *value_scales; // null: pages of T
+  void *key, *value;                        // [tokens, kv_heads, D]; written by the read
+  int64_t key_head, key_token, value_head, value_token; // element strides
+  const int *rows, *positions;              // [tokens]: sequence and position of each token
+  PageMap map;
+  int64_t tokens;
+};
+
+// Slot (row of the pages) of token t's head, or -1 if the token has none: a
+// sequence outside the table, a position outside the sequence's pages (negative
+// ones mark tokens to pass over) or a page number outside the pool.
+__device__ __forceinline__ int64_t slot_of(const PagedKVArgs &a, int64_t t, int head) {
+  const int row = a.rows[t], position = a.positions[t];
+  if (row < 0 || row >= a.map.sequences || position < 0) return -1;
+  const int index = position >> a.map.page_shift;
+  if (index >= a.map.max_pages) return -1;
+  const int page = a.map.table[(int64_t)row * a.map.max_pages + index];
+  if (page < 0 || page >= a.map.num_pages) return -1;
+  const int slot = position & ((1 << a.map.page_shift) - 1);
+  return ((((int64_t)page * a.map.kv_heads + head) << a.map.page_shift) + slot);
+}
+
+// Largest of the LANES values of an aligned group of lanes (8, 16 or 32).
+template <int LANES>
+__device__ __forceinline__ float max_over_lanes(float v) {
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  if constexpr (LANES >= 16) v = fmaxf(v, dpp_move<0x140>(v));
+  if constexpr (LANES >= 32)
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F)));
+  return v;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void store_e4m3(unsigned char *pages, unsigned char *scales, int64_t slot, int part,
+                                           const RawVec<T, 8> &raw) {
+  float x[8];
+  raw_to_f32<T, 8>(x, raw);
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, __builtin_isfinite(x[i]) ? fabsf(x[i]) : 0.f);
+  amax = max_over_lanes<D / 8>(amax);
+  const int e = scale_exponent(__builtin_bit_cast(uint32_t, amax));
+  const float inverse = exponent_to_scale(127 - e);
+  // (infinities and NaN have no scaled value: they are kept as NaN)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __builtin_isfinite(x[i]) ? x[i] * inverse : __builtin_nanf("");
+  u32x2 w;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j], x[4 * j + 1], 0, false);
+    v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2], x[4 * j + 3], v, true);
+    w[j] = (uint32_t)v;
+  }
+  if (slot >= 0) {
+    *reinterpret_cast<u32x2 *>(pages + slot * D + 8 * part) = w;
+    if (part == 0) scales[slot] = (unsigned char)(e + 127);
+  }
+}
+
+template <typename T, int D, bool E4M3>
+__global__ __launch_bounds__(kBlockThreads) void paged_kv_write_kernel(const PagedKVArgs a) {
+  constexpr int kLanes = D / 8;
+  constexpr int kRows = kBlockThreads / kLanes;
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
+  const int part = threadIdx.x % kLanes;
+  const int64_t t = row / a.map.kv_heads;
+  const int head = (int)(row - t * a.map.kv_heads);
+  if (t >= a.tokens) return; // (whole groups of lanes)
+  using V = RawVec<T, 8>;
+  const V k = *reinterpret_cast<const V *>(static_cast<const T *>(a.key) + t * a.key_token + head * a.key_head + 8 * part);
+  const V v =
+      *reinterpret_cast<const V *>(static_cast<const T *>(a.value) + t * a.value_token + head * a.value_head + 8 * part);
+  const int64_t slot = slot_of(a, t, head);
+  if constexpr (E4M3) {
+    store_e4m3<T, D>(static_cast<unsigned char *>(a.key_pages), a.key_scales, slot, part, k);
+    store_e4m3<T, D>(static_cast<unsigned char *>(a.value_pages), a.value_scales, slot, part, v);
+  } else if (slot >= 0) {
+    *reinterpret_cast<V *>(static_cast<T *>(a.key_pages) + slot * D + 8 * part) = k;
+    *reinterpret_cast<V *>(static_cast<T *>(a.value_pages) + slot * D + 8 * part) = v;
+  }
+}
+
+template <typename T, int D, bool E4M3>
+__global__ __launch_bounds__(kBlockThreads) void paged_kv_read_kernel(const PagedKVArgs a) {
+  constexpr int kLanes = D / 8;
+  constexpr int kRows = kBlockThreads / kLanes;
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
+  const int part = threadIdx.x % kLanes;
+  const int64_t t = row / a.map.kv_heads;
+  const int head = (int)(row - t * a.map.kv_heads);
+  if (t >= a.tokens) return;
+  using V = RawVec<T, 8>;
+  const int64_t slot = slot_of(a, t, head);
+  V out[2];
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const void *pages = which ? a.value_pages : a.key_pages;
+    V x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<T>(0.f); // (a token without a slot reads as zeros)
+    if (slot >= 0) {
+      if constexpr (E4M3) {
+        const u32x2 w = *reinterpret_cast<const u32x2 *>(static_cast<const unsigned char *>(pages) + slot * D + 8 * part);
+        const float scale = exponent_to_scale((which ? a.value_scales : a.key_scales)[slot]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const Pair<T> lo = e4m3_pair<false>(w[j], scale, T()), hi = e4m3_pair<true>(w[j], scale, T());
+          x[4 * j] = lo[0], x[4 * j + 1] = lo[1], x[4 * j + 2] = hi[0], x[4 * j + 3] = hi[1];
+        }
+      } else {
+        x = *reinterpret_cast<const V *>(static_cast<const T *>(pages) + slot * D + 8 * part);
+      }
+    }
+    out[which] = x;
+  }
+  const int64_t at = row * D + 8 * part; // (dense outputs)
+  *reinterpret_cast<V *>(static_cast<T *>(a.key) + at) = out[0];
+  *reinterpret_cast<V *>(static_cast<T *>(a.value) + at) = out[1];
+}
+
+template <typename T, int D, bool WRITE>
+int launch_paged_kv(const PagedKVArgs &a, hipStream_t stream) {
+  constexpr int kRows = kBlockThreads / (D / 8);
+  const dim3 grid((unsigned)((a.tokens * a.map.kv_heads + kRows - 1) / kRows));
+  if constexpr (WRITE) {
+    auto *kernel = a.key_scales ? paged_kv_write_kernel<T, D, true> : paged_kv_write_kernel<T, D, false>;
+    kernel<<<grid, dim3(kBlockThreads), 0, stream>>>(a);
+  } else {
+    auto *kernel = a.key_scales ? paged_kv_read_kernel<T, D, true> : paged_kv_read_kernel<T, D, false>;
+    kernel<<<grid, dim3(kBlockThreads), 0, stream>>>(a);
+  }
+  return check_launch(WRITE ? "paged_kv_write" : "paged_kv_read");
+}
+
+template <typename T, bool WRITE>
+int launch_paged_kv_dim(const PagedKVArgs &a, int64_t head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 64: return launch_paged_kv<T, 64, WRITE>(a, stream);
+    case 128: return launch_paged_kv<T, 128, WRITE>(a, stream);
+    default: return launch_paged_kv<T, 256, WRITE>(a, stream);
+  }
+}
+
+template <bool WRITE>
+int paged_kv(const char *name, PagedKVArgs a, int64_t sequences, int64_t max_pages, int64_t num_pages,
+             int64_t kv_heads, int64_t page_size, int64_t head_dim, int dtype, hipStream_t stream) {
+  if (a.tokens < 0) return fail(OSLO_E_BAD_ARG, "%s: negative size", name);
+  const int s = check_pages(name, a.key_pages, a.value_pages, a.key_scales, a.value_scales, a.map.table, sequences,
+                            max_pages, num_pages, kv_heads, page_size, head_dim, dtype, &a.map);
+  if (s != OSLO_OK) return s;
+  if (a.tokens == 0 || kv_heads == 0) return OSLO_OK;
+  if (!a.key || !a.value || !a.rows || !a.positions) return fail(OSLO_E_BAD_ARG, "%s: null pointer", name);
+  if (!aligned16(a.key) || !aligned16(a.value))
+    return fail(OSLO_E_UNSUPPORTED, "%s: key and value must be 16-byte aligned", name);
+  if (a.key_head < 0 || a.key_token < 0 || a.value_head < 0 || a.value_token < 0 || a.key_head % 8 ||
+      a.key_token % 8 || a.value_head % 8 || a.value_token % 8)
+    return fail(OSLO_E_UNSUPPORTED, "%s: strides must be multiples of 8 elements", name);
+  if (a.tokens > (int64_t)0x7fffffff / kv_heads)
+    return fail(OSLO_E_UNSUPPORTED, "%s: too many tokens for one launch", name);
+  if (dtype == OSLO_F16) return launch_paged_kv_dim<f16, WRITE>(a, head_dim, stream);
+  return launch_paged_kv_dim<bf16, WRITE>(a, head_dim, stream);
+}
+
+} // namespace
+} // namespace oslo
+
+extern "C" int oslo_paged_kv_write(void *key_pages, void *value_pages, uint8_t *key_scales,
+                                   uint8_t *value_scales, const void *key, const void *value,
+                                   const int32_t *sequence, const int32_t *position,
+                                   const int32_t *table, int64_t tokens, int64_t sequences,
+                                   int64_t max_pages, int64_t num_pages, int64_t kv_heads,
+                                   int64_t page_size, int64_t head_dim, const int64_t *strides,
+                                   int dtype, oslo_stream_t stream) {
+  using namespace oslo;
+  if (!strides && tokens > 0) return fail(OSLO_E_BAD_ARG, "oslo_paged_kv_write: null pointer");
+  PagedKVArgs a{};
+  a.key_pages = key_pages, a.value_pages = value_pages, a.key_scales = key_scales, a.value_scales = value_scales;
+  a.key = const_cast<void *>(key), a.value = const_cast<void *>(value);
+  if (strides) a.key_head = strides[0], a.key_token = strides[1], a.value_head = strides[2], a.value_token = strides[3];
+  a.rows = sequence, a.positions = position, a.map.table = table, a.tokens = tokens;
+  return paged_kv<true>("oslo_paged_kv_write", a, sequences, max_pages, num_pages, kv_heads, page_size, head_dim,
+                        dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int oslo_paged_kv_read(void *key, void *value, const void *key_pages,
+                                  const void *value_pages, const uint8_t *key_scales,
+                                  const uint8_t *value_scales, const int32_t *sequence,
+                                  const int32_t *position, const int32_t *table, int64_t tokens,
+                                  int64_t sequences, int64_t max_pages, int64_t num_pages,
+                                  int64_t kv_heads, int64_t page_size, int64_t head_dim, int dtype,
+                                  oslo_stream_t stream) {
+  using namespace oslo;
+  PagedKVArgs a{};
+  a.key_pages = const_cast<void *>(key_pages), a.value_pages = const_cast<void *>(value_pages);
+  a.key_scales = const_cast<uint8_t *>(key_scales), a.value_scales = const_cast<uint8_t *>(value_scales);
+  a.key = key, a.value = value;
+  a.rows = sequence, a.positions = position, a.map.table = table, a.tokens = tokens;
+  return paged_kv<false>("oslo_paged_kv_read", a, sequences, max_pages, num_pages, kv_heads, page_size, head_dim,
+                         dtype, static_cast<hipStream_t>(stream));
+}

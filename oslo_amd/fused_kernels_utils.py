@@ -682,6 +682,150 @@ class FusedPrefillAttention(object):
         return get_custom_kernels().attention_prefill_forward(query, key, value, scale, pad, window or 0)
 
 
+class _PackedAttention(torch.autograd.Function):
+    """The packed attention with its backward, which recomputes the
+    probabilities from the log-sum-exp of every row. It cannot be differentiated
+    again, and it always computes all three gradients."""
+
+    @staticmethod
+    def forward(ctx, query, key, value, packed, scale, window):
+        out, lse = get_custom_kernels().attention_packed_forward(query, key, value, packed, scale, window,
+                                                                 want_lse=True)
+        ctx.save_for_backward(query, key, value, out, lse)
+        ctx.args = (packed, float(scale), int(window))
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        query, key, value, out, lse = ctx.saved_tensors
+        packed, scale, window = ctx.args
+        dq, dk, dv = get_custom_kernels().attention_packed_backward(grad_out, query, key, value, out, lse, packed,
+                                                                    scale, window)
+        return dq, dk, dv, None, None, None
+
+
+class FusedPackedAttention(object):
+    """
+    Kernel fusion function: causal attention over packed sequences
+
+    Before fusion: pad to the longest -> Matmul -> (Scale + Mask + Softmax) -> Matmul
+    After fusion: one kernel over the tokens there are; no position sees another sequence
+
+    Not in the reference, whose attention takes padded batches
+    (oslo/models/gptj/modeling_gptj.py:936-951). ``apply`` takes query
+    [T, H, D], key and value [T, Hkv, D] (H a multiple of Hkv; views with
+    contiguous features are read where they lie), the ``PackedSequences`` of
+    the row and the scale, and returns [T, H, D]; rows behind the last sequence
+    come back as zeros. fp16 and bf16, heads of 64, 128 or 256 features, no
+    attention dropout. Differentiable: dK and dV are summed over the query
+    heads of a group inside the kernel; the same bits from run to run.
+    """
+
+    @staticmethod
+    def is_available(query, key, training=False, dropout_p=0.0):
+        return (query.is_cuda and query.dim() == 3 and key.dim() == 3 and query.dtype in (torch.half, torch.bfloat16)
+                and key.dtype == query.dtype and query.size(2) in (64, 128, 256) and key.size(2) == query.size(2)
+                and key.size(1) > 0 and query.size(1) % key.size(1) == 0 and not (training and dropout_p > 0.0))
+
+    @staticmethod
+    def apply(query, key, value, packed, scale=None, window=None):
+        """``window``: query i sees the keys i - window < s <= i of its sequence."""
+        scale = 1.0 if scale is None else scale
+        if _needs_grad(query, key, value):
+            return _PackedAttention.apply(query, key, value, packed, scale, window or 0)
+        return get_custom_kernels().attention_packed_forward(query, key, value, packed, scale, window or 0)
+
+
+def _refuse_grad(what, *tensors):
+    if _needs_grad(*tensors):
+        raise RuntimeError(f"{what} is for inference: call it under torch.no_grad()")
+
+
+class FusedPagedKV(object):
+    """
+    Kernel fusion function: new keys and values into a paged cache, and back
+
+    Before: torch.cat((past, new)) per layer and step
+    After: one launch that writes every token into its slot, in 16 or 8 bits
+
+    Not in the reference, whose cache grows by concatenation
+    (oslo/models/gptj/modeling_gptj.py:205-233). The cache is a ``PagedKV``; a
+    token goes to ``position[t]`` of ``sequence[t]`` (int32 device tensors).
+    8-bit caches keep a vector as e4m3 numbers with a power-of-two scale.
+    Tokens that name no place (a negative position, a sequence or page out of
+    range) are passed over by ``write`` and zeros for ``read``; two tokens of
+    a call must not name the same place. Inference only.
+    """
+
+    @staticmethod
+    def write(cache, key, value, sequence, position):
+        """key, value: [T, Hkv, D]."""
+        _refuse_grad("FusedPagedKV.write", key, value)
+        get_custom_kernels().paged_kv_write(cache, key, value, sequence, position)
+
+    @staticmethod
+    def read(cache, sequence, position, dtype):
+        """Returns key, value [T, Hkv, D] of ``dtype`` (fp16 or bf16)."""
+        return get_custom_kernels().paged_kv_read(cache, sequence, position, dtype)
+
+
+class FusedPagedDecodeAttention(object):
+    """
+    Kernel fusion function: the attention of a decoding step over a paged cache
+
+    Before fusion: pad to the longest -> Matmul -> (Scale + Mask + Softmax) -> Matmul
+    After fusion: one pass over the visible keys and values of each sequence
+
+    Not in the reference. ``apply`` takes one query per sequence [B, H, D], the
+    ``PagedKV`` cache (16 or 8 bits, H a multiple of its heads), the
+    sequences' lengths (int32 [B] on the device, read by the kernel, the new
+    token's position included) and an optional sliding window; it returns
+    [B, H, D]. A length of 0 gives zeros; a length or a page number that the
+    cache does not have gives NaN. Inference only.
+    """
+
+    @staticmethod
+    def is_available(query, cache, training=False, dropout_p=0.0):
+        hkv, page, d = cache.key_pages.shape[1:]
+        return (query.is_cuda and query.dim() == 3 and query.dtype in (torch.half, torch.bfloat16)
+                and (cache.quantized or cache.key_pages.dtype == query.dtype) and d in (64, 128, 256)
+                and query.size(2) == d and hkv > 0 and query.size(1) % hkv == 0
+                and 16 <= page <= 4096 and page & (page - 1) == 0 and not (training and dropout_p > 0.0)
+                and not _needs_grad(query))
+
+    @staticmethod
+    def apply(query, cache, lengths, scale=None, window=None):
+        _refuse_grad("FusedPagedDecodeAttention", query)
+        return get_custom_kernels().attention_paged_decode_forward(query, cache, lengths,
+                                                                   1.0 if scale is None else scale, window or 0)
+
+
+class FusedSampling(object):
+    """
+    Kernel fusion function: temperature, top-k, top-p and min-p, and the draw
+
+    Before fusion: divide -> topk -> sort -> softmax -> cumsum -> mask -> softmax -> multinomial
+    After fusion: one launch, a block per row
+
+    The reference samples on the framework's operators
+    (oslo/generation_utils.py). ``apply`` takes logits [B, V] (fp32,
+    fp16 or bf16) and one uniform number in [0, 1) per row (fp32 [B]) and returns
+    the int64 [B] tokens and the fp32 [B] logarithms of their probabilities
+    under the filtered distribution. Filters in that order, each on what the one
+    before has left: the ``top_k`` largest (0: all), the shortest front with
+    ``top_p`` of the mass (1: all), those with at least ``min_p`` of the largest
+    probability; equal logits go by the lower index. A temperature of 0 takes
+    the largest logit. Every setting is a number or a device tensor of one value
+    per row (fp32; ``top_k`` int32). Logits of -inf are never drawn, NaN counts
+    as -inf, a row of nothing else gives token -1.
+    """
+
+    @staticmethod
+    def apply(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        return get_custom_kernels().sample_forward(logits.detach(), uniforms, temperature, top_k, top_p, min_p)
+
+
 class FusedLinearRows(object):
     """
     Kernel fusion function: Linear + Bias + Activation for a decoding step

@@ -718,6 +718,217 @@ def attention_prefill_backward(grad_out, query, key, value, out, lse, scale, pad
     return dq, dk, dv
 
 
+# ---------------------------------------------------------------------------
+# sequences of different lengths: packed rows, the paged cache, sampling
+# ---------------------------------------------------------------------------
+
+def _packed_strided(t):
+    """t [T, heads, D] as the packed attention can read it; a copy if not."""
+    ok = t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.stride(0) >= t.shape[2] \
+        and t.data_ptr() % 16 == 0
+    return t if ok else t.contiguous()
+
+
+def _packed_args(query, key, value, packed):
+    _device_tensor(query, "query")
+    _device_tensor(key, "key", query)
+    _device_tensor(value, "value", query)
+    code = _dtype_code(query, "query")
+    _require(query.dtype in (torch.float16, torch.bfloat16), "attention_packed: fp16 or bf16 tensors")
+    _require(query.dim() == 3 and key.dim() == 3 and key.shape == value.shape,
+             "query must be [tokens, heads, D], key and value [tokens, key/value heads, D]")
+    _require(key.dtype == query.dtype and value.dtype == query.dtype, "query, key and value differ in dtype")
+    t, h, d = query.shape
+    hkv = key.shape[1]
+    _require(key.shape[0] == t and key.shape[2] == d, "query, key and value differ in tokens or features")
+    _require(hkv > 0 and h % hkv == 0 if h else True, f"{h} query heads do not share {hkv} key/value heads evenly")
+    _require(d in PREFILL_HEAD_DIMS, f"attention_packed: heads of {d} features (64, 128 or 256 are taken)")
+    _require(packed.total <= t, f"the sequences have {packed.total} tokens, the tensors {t}")
+    _require(packed.blocks.device == query.device, f"the sequences are on {packed.blocks.device}, query on {query.device}")
+    return code
+
+
+def _token_strides(tensors):
+    strides = (ctypes.c_int64 * (2 * len(tensors)))()
+    for i, t in enumerate(tensors):
+        strides[2 * i], strides[2 * i + 1] = t.stride(1), t.stride(0)
+    return strides
+
+
+def _packed_empty(tokens, heads, d, packed, like):
+    """An uninitialised [tokens, heads, D] whose rows behind the last sequence are zeros."""
+    out = torch.empty((tokens, heads, d), dtype=like.dtype, device=like.device)
+    if packed.total < tokens:
+        out[packed.total:].zero_()
+    return out
+
+
+def attention_packed_forward(query, key, value, packed, scale, window=0, want_lse=False):
+    """Causal attention over the sequences ``packed`` (a ``PackedSequences``)
+    laid one behind the other: query [T, H, D], key and value [T, Hkv, D]
+    fp16/bf16 views (features contiguous), H a multiple of Hkv. Returns
+    [T, H, D] (rows behind the last sequence: zeros), with ``want_lse`` also the
+    fp32 [H, T] log2-sum-exp that ``attention_packed_backward`` takes."""
+    code = _packed_args(query, key, value, packed)
+    t, h, d = query.shape
+    q, k, v = (_packed_strided(x) for x in (query, key, value))
+    out = _packed_empty(t, h, d, packed, query)
+    lse = torch.empty((h, t), dtype=torch.float32, device=query.device) if want_lse else None
+    if packed.total and h:
+        with _on_device(q):
+            _lib.check(_lib.load().oslo_attention_packed_fwd(
+                _ptr(out), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), _ptr(packed.blocks[0]), packed.blocks.shape[1],
+                float(scale), t, packed.max_length, h, k.shape[1], d, int(window), _token_strides((q, k, v, out)),
+                code, _stream(q)))
+    return (out, lse) if want_lse else out
+
+
+def attention_packed_backward(grad_out, query, key, value, out, lse, packed, scale, window=0):
+    """Gradients of ``attention_packed_forward`` with respect to query, key and
+    value (dense; rows behind the last sequence: zeros)."""
+    code = _packed_args(query, key, value, packed)
+    for what, x in (("grad_out", grad_out), ("out", out)):
+        _device_tensor(x, what, query)
+        _require(x.shape == query.shape and x.dtype == query.dtype, f"{what} must be like query")
+    _device_tensor(lse, "lse", query)
+    t, h, d = query.shape
+    hkv = key.shape[1]
+    _require(lse.dtype == torch.float32 and tuple(lse.shape) == (h, t) and lse.is_contiguous(),
+             "lse must be the fp32 [H, T] tensor of the forward")
+    q, k, v, o, g = (_packed_strided(x) for x in (query, key, value, out, grad_out))
+    dq = _packed_empty(t, h, d, packed, query)
+    dk, dv = (_packed_empty(t, hkv, d, packed, query) for _ in range(2))
+    if packed.total and h:
+        lib = _lib.load()
+        ws = torch.empty(lib.oslo_attention_packed_bwd_workspace_bytes(t, h) // 4, dtype=torch.float32,
+                         device=query.device)
+        with _on_device(q):
+            _lib.check(lib.oslo_attention_packed_bwd(
+                _ptr(dq), _ptr(dk), _ptr(dv), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(ws),
+                _ptr(packed.blocks[0]), _ptr(packed.blocks[1]), packed.blocks.shape[1], float(scale), t,
+                packed.max_length, h, hkv, d, int(window), _token_strides((q, k, v, o, g, dq, dk, dv)), code,
+                _stream(q)))
+    return dq, dk, dv
+
+
+def _index_tensor(t, what, like, length):
+    _device_tensor(t, what, like)
+    _require(t.dtype == torch.int32 and tuple(t.shape) == (length,), f"{what} must be int32 [{length}]")
+    return t.contiguous()
+
+
+def _cache_args(cache, like, what):
+    """What every call over a ``PagedKV`` passes on: its pointers and sizes."""
+    _require(cache.key_pages.device == like.device, f"the cache is on {cache.key_pages.device}, {what} on {like.device}")
+    _require(like.dtype in (torch.float16, torch.bfloat16), f"{what}: fp16 or bf16, got {like.dtype}")
+    _require(cache.quantized or cache.key_pages.dtype == like.dtype,
+             f"{what} is {like.dtype}, the cache {cache.key_pages.dtype}")
+    pages, hkv, page, d = cache.key_pages.shape
+    return (_ptr(cache.key_pages), _ptr(cache.value_pages), _ptr(cache.key_scales), _ptr(cache.value_scales)), \
+        (cache.table.shape[0], cache.table.shape[1], pages), (hkv, page, d)
+
+
+def paged_kv_write(cache, key, value, sequence, position):
+    """key, value [T, Hkv, D] -> position[t] (int32 [T]) of sequence[t] (int32
+    [T]) of the ``PagedKV`` cache. Tokens that name no place of the cache (a
+    negative position, a sequence or page out of range) are passed over."""
+    _device_tensor(key, "key")
+    _device_tensor(value, "value", key)
+    code = _dtype_code(key, "key")
+    pointers, counts, (hkv, page, d) = _cache_args(cache, key, "key")
+    _require(key.dim() == 3 and tuple(key.shape[1:]) == (hkv, d), f"key must be [tokens, {hkv}, {d}]")
+    _require(value.shape == key.shape and value.dtype == key.dtype, "key and value differ in shape or dtype")
+    t = key.shape[0]
+    sequence, position = _index_tensor(sequence, "sequence", key, t), _index_tensor(position, "position", key, t)
+    k, v = _packed_strided(key), _packed_strided(value)
+    with _on_device(k):
+        _lib.check(_lib.load().oslo_paged_kv_write(
+            *pointers, _ptr(k), _ptr(v), _ptr(sequence), _ptr(position), _ptr(cache.table), t, *counts, hkv, page, d,
+            _token_strides((k, v)), code, _stream(k)))
+
+
+def paged_kv_read(cache, sequence, position, dtype):
+    """The keys and values of the tokens (sequence[t], position[t]), each
+    [T, Hkv, D] of ``dtype``; zeros for tokens that name no place."""
+    _device_tensor(sequence, "sequence", cache.key_pages)
+    _require(sequence.dim() == 1, "sequence must be int32 [tokens]")
+    t = sequence.shape[0]
+    sequence, position = (_index_tensor(x, what, cache.key_pages, t) for x, what in
+                          ((sequence, "sequence"), (position, "position")))
+    pages, hkv, page, d = cache.key_pages.shape
+    key, value = (torch.empty((t, hkv, d), dtype=dtype, device=sequence.device) for _ in range(2))
+    code = _dtype_code(key, "dtype")
+    pointers, counts, _ = _cache_args(cache, key, "dtype")
+    with _on_device(key):
+        _lib.check(_lib.load().oslo_paged_kv_read(
+            _ptr(key), _ptr(value), *pointers, _ptr(sequence), _ptr(position), _ptr(cache.table), t, *counts, hkv,
+            page, d, code, _stream(key)))
+    return key, value
+
+
+def attention_paged_decode_forward(query, cache, lengths, scale, window=0):
+    """query [B, H, D], one new token per sequence of the ``PagedKV`` cache;
+    lengths int32 [B] on the device: sequence b's visible positions are those
+    below lengths[b] (the last ``window`` of them). Returns [B, H, D]."""
+    _device_tensor(query, "query")
+    code = _dtype_code(query, "query")
+    pointers, counts, (hkv, page, d) = _cache_args(cache, query, "query")
+    _require(query.dim() == 3 and query.shape[2] == d, f"query must be [sequences, heads, {d}]")
+    b, h, _ = query.shape
+    _require(b == counts[0], f"{b} queries for a table of {counts[0]} sequences")
+    _require(hkv > 0 and h % hkv == 0, f"{h} query heads do not share {hkv} key/value heads evenly")
+    lengths = _index_tensor(lengths, "lengths", query, b)
+    q = query
+    if not (q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0 and q.data_ptr() % 16 == 0):
+        q = q.contiguous()
+    lib = _lib.load()
+    nbytes = lib.oslo_attention_paged_decode_workspace_bytes(b, h, hkv, d, counts[1] * page, int(window))
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
+    out = torch.empty((b, h, d), dtype=q.dtype, device=q.device)
+    strides = (ctypes.c_int64 * 2)(q.stride(0), q.stride(1))
+    with _on_device(q):
+        _lib.check(lib.oslo_attention_paged_decode_fwd(
+            _ptr(out), _ptr(q), *pointers, _ptr(cache.table), _ptr(lengths), _ptr(ws), float(scale), *counts, h, hkv,
+            page, d, int(window), strides, code, _stream(q)))
+    return out
+
+
+def _row_setting(value, what, dtype, rows, like):
+    """(pointer holder, number) of a sampling setting: a tensor of one value per
+    row, or a number for all."""
+    if isinstance(value, torch.Tensor):
+        _device_tensor(value, what, like)
+        _require(value.dtype == dtype and tuple(value.shape) == (rows,), f"{what} must be a number or {dtype} [{rows}]")
+        return value.contiguous(), 0
+    return None, value
+
+
+def sample_forward(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """logits [B, V] (fp32, fp16 or bf16), uniforms fp32 [B] in [0, 1) -> int64
+    [B] tokens and the fp32 [B] logarithms of their shares. Every setting is a
+    number or a device tensor of one value per row (fp32; top_k int32)."""
+    _device_tensor(logits, "logits")
+    code = _dtype_code(logits, "logits")
+    _require(logits.dim() == 2, "logits must be [rows, vocabulary]")
+    rows, vocab = logits.shape
+    _device_tensor(uniforms, "uniforms", logits)
+    _require(uniforms.dtype == torch.float32 and tuple(uniforms.shape) == (rows,), f"uniforms must be fp32 [{rows}]")
+    temperature, temperature_all = _row_setting(temperature, "temperature", torch.float32, rows, logits)
+    top_k, top_k_all = _row_setting(top_k, "top_k", torch.int32, rows, logits)
+    top_p, top_p_all = _row_setting(top_p, "top_p", torch.float32, rows, logits)
+    min_p, min_p_all = _row_setting(min_p, "min_p", torch.float32, rows, logits)
+    x = logits if logits.stride(1) == 1 and (rows <= 1 or logits.stride(0) >= 0) else logits.contiguous()
+    uniforms = uniforms.contiguous()
+    tokens = torch.empty((rows,), dtype=torch.int64, device=x.device)
+    logprobs = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    with _on_device(x):
+        _lib.check(_lib.load().oslo_sample(
+            _ptr(tokens), _ptr(logprobs), _ptr(x), _ptr(uniforms), _ptr(temperature), float(temperature_all),
+            _ptr(top_k), int(top_k_all), _ptr(top_p), float(top_p_all), _ptr(min_p), float(min_p_all), rows, vocab,
+            x.stride(0), code, _stream(x)))
+    return tokens, logprobs
+
+
 def rotary_qkv_forward(query, key, value, sin, cos, rotary_dim, offset=0):
     """query, key, value: [B, S, H, D] (any may be None); sin, cos: fp32
     [positions, rotary_dim/2]. Returns the three tensors as [B, H, S, D], query

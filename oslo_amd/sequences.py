@@ -1,0 +1,118 @@
+"""Sequences of different lengths: how they are packed into one row of tokens
+(``PackedSequences``), and the paged key/value cache they are decoded over
+(``PagedKV``). No counterpart in the reference, whose models take padded batches
+and whose cache grows by concatenation
+(oslo/models/gptj/modeling_gptj.py:205-233)."""
+
+import numpy as np
+import torch
+
+PACKED_BLOCK = 128  # positions of a sequence one block of the attention kernels takes
+
+
+class PackedSequences(object):
+    """Sequences of ``lengths`` tokens (host integers, zero allowed) laid one
+    behind the other along one row. Made once per batch, before any capture,
+    and shared by every layer and by the backward: it holds, on ``device``, the
+    list of 128-position blocks the attention kernels take their work from
+    (``blocks``: int32 [2, n, 4]; the blocks with most keys first, then those
+    with most queries left first)."""
+
+    def __init__(self, lengths, device):
+        lengths = [int(n) for n in lengths]
+        if any(n < 0 for n in lengths):
+            raise ValueError("PackedSequences: lengths must not be negative")
+        self.lengths = tuple(lengths)
+        self.total = sum(lengths)
+        self.max_length = max(lengths, default=0)
+        if self.total >= 2 ** 31:
+            raise ValueError("PackedSequences: more than 2^31 - 1 tokens")
+        n = np.asarray(lengths, dtype=np.int64)
+        self._starts = np.concatenate([[0], np.cumsum(n)[:-1]]).astype(np.int64) if len(n) else n
+        counts = -(-n // PACKED_BLOCK)
+        owner = np.repeat(np.arange(len(n)), counts)
+        block = np.arange(len(owner)) - np.repeat(np.cumsum(counts) - counts, counts)
+        entries = np.zeros((len(owner), 4), dtype=np.int32)
+        entries[:, 0], entries[:, 1], entries[:, 2] = self._starts[owner], n[owner], block
+        keys = np.minimum((block + 1) * PACKED_BLOCK, n[owner])
+        queries = n[owner] - block * PACKED_BLOCK
+        order = [np.argsort(-keys, kind="stable"), np.argsort(-queries, kind="stable")]
+        self.blocks = torch.from_numpy(np.stack([entries[o] for o in order])).to(device)
+        self._positions = self._sequence = None
+
+    @property
+    def device(self):
+        return self.blocks.device
+
+    def _per_token(self, values):
+        return torch.from_numpy(values.astype(np.int32)).to(self.device)
+
+    @property
+    def positions(self):
+        """int32 [total] on the device: each token's position in its own sequence."""
+        if self._positions is None:
+            n = np.asarray(self.lengths, dtype=np.int64)
+            self._positions = self._per_token(np.arange(self.total) - np.repeat(self._starts, n))
+        return self._positions
+
+    @property
+    def sequence(self):
+        """int32 [total] on the device: the sequence each token belongs to."""
+        if self._sequence is None:
+            self._sequence = self._per_token(np.repeat(np.arange(len(self.lengths)), self.lengths))
+        return self._sequence
+
+    def last_tokens(self):
+        """int64 [sequences] on the device: the row of each sequence's last token
+        (sequences must not be empty)."""
+        if any(n == 0 for n in self.lengths):
+            raise ValueError("PackedSequences: an empty sequence has no last token")
+        return torch.from_numpy(self._starts + np.asarray(self.lengths, dtype=np.int64) - 1).to(self.device)
+
+
+class PagedKV(object):
+    """One layer's key/value cache in pages: ``key_pages`` and ``value_pages``
+    [num_pages, key/value heads, page_size, head_dim], and ``table`` int32
+    [sequences, max_pages], the page that holds positions [i * page_size, (i + 1)
+    * page_size) of each sequence. fp16 or bf16; or 8-bit (``float8_e4m3fn``) with
+    ``key_scales`` and ``value_scales`` uint8 [num_pages, heads, page_size]: the
+    power-of-two scale of each slot's vector, as its exponent + 127."""
+
+    def __init__(self, key_pages, value_pages, table, key_scales=None, value_scales=None):
+        if key_pages.dim() != 4 or key_pages.shape != value_pages.shape or key_pages.dtype != value_pages.dtype:
+            raise ValueError("PagedKV: pages must be two [pages, heads, page_size, head_dim] tensors alike")
+        if not (key_pages.is_contiguous() and value_pages.is_contiguous()):
+            raise ValueError("PagedKV: pages must be contiguous")
+        if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous():
+            raise ValueError("PagedKV: the table must be a contiguous int32 [sequences, max_pages] tensor")
+        self.quantized = key_pages.dtype == torch.float8_e4m3fn
+        if not self.quantized and key_pages.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"PagedKV: pages of fp16, bf16 or float8_e4m3fn, not {key_pages.dtype}")
+        scales = (key_scales, value_scales)
+        if self.quantized:
+            if not all(isinstance(s, torch.Tensor) and s.dtype == torch.uint8 and s.shape == key_pages.shape[:3]
+                       and s.is_contiguous() for s in scales):
+                raise ValueError("PagedKV: 8-bit pages need contiguous uint8 [pages, heads, page_size] scales")
+        elif any(s is not None for s in scales):
+            raise ValueError("PagedKV: scales go with 8-bit pages")
+        tensors = [value_pages, table] + [s for s in scales if s is not None]
+        if any(t.device != key_pages.device for t in tensors):
+            raise ValueError("PagedKV: pages, table and scales must be on one device")
+        self.key_pages, self.value_pages, self.table = key_pages, value_pages, table
+        self.key_scales, self.value_scales = scales
+
+    @property
+    def page_size(self):
+        return self.key_pages.shape[2]
+
+    @classmethod
+    def allocate(cls, table, num_pages, kv_heads, page_size, head_dim, dtype, device, quantized=False):
+        """An empty cache of ``num_pages`` pages under ``table`` (layers that grow
+        together share one table)."""
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        if not quantized:
+            return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
+                       table)
+        pages = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+        scales = [torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2)]
+        return cls(*pages, table, *scales)

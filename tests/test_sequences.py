@@ -1,0 +1,164 @@
+"""Sequences of different lengths, the host side: the list of blocks the packed
+attention takes its work from, the paged cache's checks, and what the entry
+points refuse before they launch anything."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oslo_amd import PackedSequences, PagedKV, kernels
+from oslo_amd import _lib
+
+
+@pytest.mark.parametrize("lengths", [[], [0], [1], [0, 5, 0, 128, 129, 127, 0], [300, 31, 33, 64, 1000]],
+                         ids=lambda v: "-".join(map(str, v)) or "none")
+def test_blocks_cover_every_token_once(lengths):
+    packed = PackedSequences(lengths, "cpu")
+    assert packed.total == sum(lengths) and packed.max_length == max(lengths, default=0)
+    for which, work in ((0, lambda s, n, b: min(n, 128 * (b + 1))), (1, lambda s, n, b: n - 128 * b)):
+        seen = np.zeros(packed.total, dtype=int)
+        amounts = []
+        for start, n, b, _ in packed.blocks[which].tolist():
+            assert 128 * b < n
+            seen[start + 128 * b:start + min(n, 128 * (b + 1))] += 1
+            amounts.append(work(start, n, b))
+        assert (seen == 1).all()
+        assert amounts == sorted(amounts, reverse=True)
+    assert packed.positions.tolist() == [p for n in lengths for p in range(n)]
+    assert packed.sequence.tolist() == [i for i, n in enumerate(lengths) for _ in range(n)]
+    assert packed.positions.dtype == torch.int32 and packed.sequence.dtype == torch.int32
+
+
+def test_last_tokens():
+    assert PackedSequences([3, 1, 4], "cpu").last_tokens().tolist() == [2, 3, 7]
+    with pytest.raises(ValueError):
+        PackedSequences([3, 0], "cpu").last_tokens()
+    with pytest.raises(ValueError):
+        PackedSequences([3, -1], "cpu")
+    with pytest.raises(ValueError):
+        PackedSequences([2 ** 31], "cpu")
+
+
+def test_paged_kv_checks_its_tensors():
+    pages = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    table = torch.zeros((3, 2), dtype=torch.int32)
+    cache = PagedKV(pages, pages.clone(), table)
+    assert not cache.quantized and cache.page_size == 16
+    with pytest.raises(ValueError):
+        PagedKV(pages, pages[:3], table)
+    with pytest.raises(ValueError):
+        PagedKV(pages, pages.half(), table)
+    with pytest.raises(ValueError):
+        PagedKV(pages.float(), pages.float(), table)
+    with pytest.raises(ValueError):
+        PagedKV(pages.transpose(1, 2), pages.transpose(1, 2), table)
+    with pytest.raises(ValueError):
+        PagedKV(pages, pages.clone(), table.long())
+    with pytest.raises(ValueError):
+        PagedKV(pages, pages.clone(), table, torch.zeros((4, 2, 16), dtype=torch.uint8),
+                torch.zeros((4, 2, 16), dtype=torch.uint8))
+    eight = pages.to(torch.float8_e4m3fn)
+    scales = torch.full((4, 2, 16), 127, dtype=torch.uint8)
+    assert PagedKV(eight, eight.clone(), table, scales, scales.clone()).quantized
+    with pytest.raises(ValueError):
+        PagedKV(eight, eight.clone(), table)
+    with pytest.raises(ValueError):
+        PagedKV(eight, eight.clone(), table, scales, scales[:, :1])
+
+
+def test_operators_reject_host_tensors():
+    q = torch.zeros((4, 2, 64), dtype=torch.bfloat16)
+    packed = PackedSequences([4], "cpu")
+    table = torch.zeros((4, 1), dtype=torch.int32)
+    pages = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    cache = PagedKV(pages, pages.clone(), table)
+    index = torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: kernels.attention_packed_forward(q, q, q, packed, 1.0),
+                 lambda: kernels.paged_kv_write(cache, q, q, index, index),
+                 lambda: kernels.paged_kv_read(cache, index, index, torch.bfloat16),
+                 lambda: kernels.attention_paged_decode_forward(q, cache, index, 1.0),
+                 lambda: kernels.sample_forward(torch.zeros((2, 8)), torch.zeros(2))):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def test_entry_points_screen_their_arguments():
+    """Every call here fails, or has nothing to do, before any pointer is followed."""
+    lib = _lib.load()
+    null, one, odd = ctypes.c_void_p(0), ctypes.c_void_p(16), ctypes.c_void_p(24)
+
+    def strides(*pairs):
+        return (ctypes.c_int64 * len(pairs))(*pairs)
+
+    # packed attention: 40 tokens, 4 heads on 2, 64 features
+    good = strides(64, 256, 64, 128, 64, 128, 64, 256)
+
+    def packed(blocks=one, n=1, scale=0.125, tokens=40, longest=40, heads=4, kv=2, d=64, window=0, st=good, dtype=2,
+               out=one, q=one):
+        return lib.oslo_attention_packed_fwd(out, null, q, one, one, blocks, n, scale, tokens, longest, heads, kv, d,
+                                             window, st, dtype, null)
+    assert packed(n=-1) == -1 and packed(tokens=-1) == -1 and packed(window=-1) == -1
+    assert packed(dtype=0) == -2 and packed(dtype=7) == -1
+    assert packed(d=48) == -2
+    assert packed(scale=0.0) == -1 and packed(scale=float("nan")) == -1
+    assert packed(heads=5) == -1 and packed(kv=0) == -1
+    assert b"share" in lib.oslo_last_error()
+    assert packed(longest=41) == -1 and packed(longest=0) == -1
+    assert packed(blocks=null) == -1 and packed(q=null) == -1 and packed(out=odd) == -2
+    assert packed(st=strides(64, 256, 64, 128, 64, 128, 64, 32)) == -2      # token stride below head_dim
+    assert packed(st=strides(64, 260, 64, 128, 64, 128, 64, 256)) == -2     # not a multiple of 8
+    assert packed(st=strides(64, 2 ** 30, 64, 128, 64, 128, 64, 256)) == -2  # a sequence of a head over 2 GiB
+    assert packed(tokens=2 ** 31, longest=40) == -2
+    assert packed(heads=2 ** 17, kv=1, st=good) == -2
+    assert packed(n=0) == 0 and packed(tokens=0) == 0 and packed(heads=0, kv=0) == 0
+    assert lib.oslo_attention_packed_bwd_workspace_bytes(40, 4) == 640
+    assert lib.oslo_attention_packed_bwd_workspace_bytes(0, 4) == 0
+    good16 = strides(*(list(good[:8]) + [64, 256, 64, 256, 64, 128, 64, 128]))
+
+    def packed_bwd(ws=one, keys=one, lse=one, dq=one):
+        return lib.oslo_attention_packed_bwd(dq, one, one, one, one, one, one, one, lse, ws, one, keys, 1, 0.125, 40, 40,
+                                             4, 2, 64, 0, good16, 2, null)
+    assert packed_bwd(ws=null) == -1 and packed_bwd(keys=null) == -1 and packed_bwd(lse=null) == -1
+    assert packed_bwd(ws=odd) == -2 and packed_bwd(dq=odd) == -2
+
+    # paged cache: 3 sequences of 5 pages, a pool of 20, 2 heads, pages of 16, 64 features
+    st4 = strides(64, 128, 64, 128)
+
+    def write(kp=one, vp=one, ks=null, vs=null, k=one, seq=one, table=one, tokens=7, page=16, d=64, dtype=2, st=st4,
+              max_pages=5):
+        return lib.oslo_paged_kv_write(kp, vp, ks, vs, k, one, seq, one, table, tokens, 3, max_pages, 20, 2, page, d,
+                                       st, dtype, null)
+    assert write(tokens=-1) == -1 and write(page=24) == -2 and write(page=8) == -2 and write(page=8192) == -2
+    assert write(d=80) == -2 and write(dtype=0) == -2 and write(dtype=9) == -1
+    assert write(ks=one) == -1 and b"together" in lib.oslo_last_error()
+    assert write(kp=null) == -1 and write(table=null) == -1 and write(k=null) == -1 and write(seq=null) == -1
+    assert write(kp=odd) == -2 and write(k=odd) == -2 and write(ks=odd, vs=one) == -2
+    assert write(st=strides(60, 128, 64, 128)) == -2 and write(st=None) == -1
+    assert write(max_pages=2 ** 26) == -2
+    assert write(tokens=0) == 0
+    assert lib.oslo_paged_kv_read(null, one, one, one, null, null, one, one, one, 7, 3, 5, 20, 2, 16, 64, 2, null) == -1
+    assert lib.oslo_paged_kv_read(one, one, one, one, null, null, one, one, one, 0, 3, 5, 20, 2, 16, 64, 2, null) == 0
+
+    def decode(out=one, q=one, lengths=one, ws=one, scale=0.125, seqs=3, heads=4, kv=2, window=0, dtype=2, d=64,
+               max_pages=5, num_pages=20, st=strides(64, 256)):
+        return lib.oslo_attention_paged_decode_fwd(out, q, one, one, null, null, one, lengths, ws, scale, seqs,
+                                                   max_pages, num_pages, heads, kv, 16, d, window, st, dtype, null)
+    assert decode(heads=-1) == -1 and decode(window=-1) == -1 and decode(scale=-1.0) == -1
+    assert decode(heads=5) == -1 and decode(dtype=0) == -2 and decode(d=32) == -2
+    assert decode(lengths=null) == -1 and decode(out=odd) == -2 and decode(st=strides(4, 256)) == -2
+    assert decode(max_pages=0) == -1 and decode(num_pages=0) == -1
+    assert decode(max_pages=4096, ws=null) == -1 and b"workspace" in lib.oslo_last_error()
+    assert decode(seqs=0) == 0 and decode(heads=0) == 0
+    assert lib.oslo_attention_paged_decode_workspace_bytes(3, 5, 2, 64, 4096, 0) == 0
+
+    # sampling
+    def sample(tokens=one, logits=one, t=1.0, k=0, p=1.0, m=0.0, rows=2, vocab=50, dtype=0):
+        return lib.oslo_sample(tokens, null, logits, one, null, t, null, k, null, p, null, m, rows, vocab, vocab, dtype,
+                               null)
+    assert sample(t=-0.5) == -1 and sample(t=float("nan")) == -1 and sample(k=-1) == -1
+    assert sample(p=-0.1) == -1 and sample(m=1.5) == -1 and sample(m=-0.1) == -1
+    assert sample(vocab=0) == -1 and sample(vocab=2 ** 24 + 1) == -2 and sample(rows=-1) == -1
+    assert sample(dtype=5) == -1 and sample(tokens=null) == -1 and sample(logits=null) == -1
+    assert sample(rows=0) == 0
