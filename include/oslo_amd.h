@@ -732,7 +732,7 @@ int oslo_attention_paged_decode_fwd(void *out, const void *q,
  * Every setting is a number of the call or, where the pointer is given, one per
  * row (fp32, top_k int32). Masses are summed as whole multiples of
  * 2^(ceil(log2 vocab) - 62) of the largest: the token does not depend on the order of
- * a sum. vocab up to 2^24. No workspace.
+ * a sum. vocab up to 500000. No workspace.
  * The reference samples on the framework's operators after sorting
  * (oslo/generation_utils.py).
  */

@@ -17,11 +17,23 @@
 // times finer than a 32-bit sum). Sums of whole numbers are exact in any order:
 // histograms may use atomics and every run gives the same token.
 //
-// One block of 1024 threads takes a row.
-// Every filter is a selection "where does the running weight along the order
-// reach a target": a histogram over 2048 steps of the distance to the largest
-// logit finds the step, three more over the bits of the logits inside that step
-// find the logit.
+// One block of 1024 threads takes a row and holds it in registers and LDS (53248
+// logits of 32 bits; what exceeds them is read again), so memory is read once. What costs the
+// time then is arithmetic, thirty instructions a logit, and barriers:
+//  - top-k goes first: a histogram of the threads' own maxima gives a bound that
+//    at least k logits reach and few exceed. They go into a list in LDS, which is all
+//    the rest looks at; up to 512 of them are ranked by counting, without a sort.
+//  - top-p over a whole row: the logits are counted over 2048 steps of the distance to
+//    the largest one. Masses inside a step differ by 0.9 %, so the counts place the border
+//    of a share p to 0.9 % p (1 - p) of the mass, a step or a few. The one exact pass
+//    then sums all masses, sums those in front of that window by segments of the row, and
+//    lists the logits in the window; the exact sums say whether the border really is among the listed ones
+//    (else an exact search finds it: the hint never decides). The listed ones are
+//    ranked.
+//  - the draw finds the segment in which the running mass passes its target, and
+//    looks inside it.
+// Windows too full for the list (equal logits by the thousand) are searched by
+// histograms over the bits of the logits.
 
 #include "common.hpp"
 
@@ -59,36 +71,25 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-
-// 2^y for y <= 0: y = n + f with |f| <= 1/2, 2^f = e^(f ln 2) by its Taylor series to the
-// eleventh power (the next term is below 2^-46 of the result), times 2^n.
-__device__ __forceinline__ double exp2_of(double y) {
-  if (!(y > -1100.0)) return 0.0; // (below the smallest double)
-  const double n = __builtin_rint(y);
-  const double z = (y - n) * 0.69314718055994530942;
-  double s = 1.0 / 39916800.0;
-  s = __builtin_fma(s, z, 1.0 / 3628800.0);
-  s = __builtin_fma(s, z, 1.0 / 362880.0);
-  s = __builtin_fma(s, z, 1.0 / 40320.0);
-  s = __builtin_fma(s, z, 1.0 / 5040.0);
-  s = __builtin_fma(s, z, 1.0 / 720.0);
-  s = __builtin_fma(s, z, 1.0 / 120.0);
-  s = __builtin_fma(s, z, 1.0 / 24.0);
-  s = __builtin_fma(s, z, 1.0 / 6.0);
-  s = __builtin_fma(s, z, 0.5);
-  s = __builtin_fma(s, z, 1.0);
-  s = __builtin_fma(s, z, 1.0);
-  return __builtin_ldexp(s, (int)n);
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-__device__ __forceinline__ u64 shfl_xor_u64(u64 v, int mask) {
-  const uint32_t lo = __shfl_xor((uint32_t)v, mask, kWave), hi = __shfl_xor((uint32_t)(v >> 32), mask, kWave);
-  return (u64)hi << 32 | lo;
-}
-__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+// 2^(i / 1024), i = 0 .. 1023, by the Taylor series of e^(i / 1024 ln 2) (to the
+// eighteenth power: below 2^-60 of the result); once per block.
+constexpr int kTable = 1024;
+__device__ __forceinline__ double table_entry(int i) {
+  const double z = (double)i * (0.69314718055994530942 / kTable);
+  double s = 1.0;
 #pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) v += shfl_xor_u64(v, d);
-  return v;
+  for (int n = 18; n >= 1; --n) s = __builtin_fma(s * z, 1.0 / n, 1.0);
+  return s;
+}
+
+// The largest float below x (x > next_below(y) just where x >= y); -inf stays.
+__device__ __forceinline__ float next_below(float x) {
+  if (x == -INFINITY) return x;
+  return key_value((x == 0.f ? 0x7fffffffu : order_key(x)) - 1); // (0 and -0 are one number)
 }
 __device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) {
   const uint32_t lo = __shfl_up((uint32_t)v, d, kWave), hi = __shfl_up((uint32_t)(v >> 32), d, kWave);
@@ -103,100 +104,206 @@ __device__ __forceinline__ u64 wave_scan_u64(u64 v, int lane) {
   }
   return v;
 }
+template <int CTRL>
+__device__ __forceinline__ u64 dpp_u64(u64 v) { // (lanes that receive nothing get 0)
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xf, 0xf, true);
+  return (u64)hi << 32 | lo;
+}
+// Sum over the wave, for every lane: rows of 16 on the vector ALU, the four rows by lane reads.
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+  v += dpp_u64<0xB1>(v);
+  v += dpp_u64<0x4E>(v);
+  v += dpp_u64<0x141>(v);
+  v += dpp_u64<0x140>(v);
+  u64 sum = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    sum += (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 16 * r) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 16 * r);
+  return sum;
+}
 
-struct SampleLds {
+constexpr int kListed = 2048; // logits the list in LDS holds
+constexpr int kRanked = 512;  // ... of which so many are ranked by counting
+
+struct alignas(16) SampleLds {
   u64 bins[kBins];
+  u64 segments[kBins];
+  u64 list[kListed]; // order_key(logit) << 32 | ~index: distinct, and in the filters' order
+  u64 ranked[kRanked];
+  double table[kTable];
   u64 wave_sums[kWaves];
   float wave_max[kWaves], wave_min[kWaves];
-  u64 found_before; // results of a search, written by the one thread that finds them
+  u64 found_before, found_value; // results of a search, written by the one thread that finds them
   int found_at;
-  int found_index;
-  double found_mass;
+  int listed;
+  uint32_t bound;
 };
+__device__ __forceinline__ u64 list_entry(float x, int index) {
+  return (u64)order_key(x) << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ float entry_logit(u64 e) { return key_value((uint32_t)(e >> 32)); }
+__device__ __forceinline__ int entry_index(u64 e) { return (int)~(uint32_t)e; }
 
-// In bins[0 .. count) (count a multiple of the block or below it): the first bin
-// at which the running sum reaches `target`, and the sum before it. Every thread
-// gets the answer; the sum of all bins must reach the target.
-__device__ __forceinline__ void find_bin(SampleLds &lds, int count, u64 target, int &bin, u64 &before) {
+// A running sum over bins[0 .. kBins): each thread's share (consecutive bins), what
+// lies before it, and the total. The bins must be complete (a barrier has passed).
+constexpr int kBinsEach = kBins / kThreads;
+struct BinScan {
+  u64 before, mine, total;
+};
+__device__ __forceinline__ BinScan scan_bins(SampleLds &lds, const u64 *bins) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  const int per = (count + kThreads - 1) / kThreads; // consecutive bins of a thread
-  u64 mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b < count) mine += lds.bins[b];
-  }
-  const u64 upto = wave_scan_u64(mine, lane);
+  BinScan s;
+  s.mine = 0;
+#pragma unroll
+  for (int i = 0; i < kBinsEach; ++i) s.mine += bins[tid * kBinsEach + i];
+  const u64 upto = wave_scan_u64(s.mine, lane);
   if (lane == kWave - 1) lds.wave_sums[wave] = upto;
   __syncthreads();
-  u64 run = upto - mine;
-  for (int w = 0; w < wave; ++w) run += lds.wave_sums[w];
-  if (run < target && run + mine >= target) { // exactly one thread
-    for (int i = 0; i < per; ++i) {
-      const int b = tid * per + i;
-      const u64 v = lds.bins[b];
-      if (run + v >= target) {
-        lds.found_at = b;
+  s.before = upto - s.mine;
+  s.total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const u64 v = lds.wave_sums[w];
+    if (w < wave) s.before += v;
+    s.total += v;
+  }
+  return s;
+}
+// The first bin at which the running sum reaches `target` (0 < target <= total), the
+// sum before it and its own value, for every thread.
+struct Found {
+  int at;
+  u64 before, value;
+};
+__device__ __forceinline__ int tid_bin(int i) { return (int)threadIdx.x * kBinsEach + i; }
+__device__ __forceinline__ Found find_bin(SampleLds &lds, const u64 *bins, const BinScan &s, u64 target) {
+  u64 run = s.before;
+  if (run < target && run + s.mine >= target) { // exactly one thread
+#pragma unroll
+    for (int i = 0; i < kBinsEach; ++i) {
+      const u64 v = bins[tid_bin(i)];
+      if (run < target && run + v >= target) {
+        lds.found_at = tid_bin(i);
         lds.found_before = run;
-        break;
+        lds.found_value = v;
       }
       run += v;
     }
   }
   __syncthreads();
-  bin = lds.found_at;
-  before = lds.found_before;
+  Found f;
+  f.at = lds.found_at, f.before = lds.found_before, f.value = lds.found_value;
+  __syncthreads(); // (the bins and the results may be written again)
+  return f;
 }
 
+// Chunks (1024 threads x 16 bytes) of a row that the registers hold, and the most
+// that LDS holds behind them (with the tables above, 157 of a CU's 160 KiB).
+constexpr int kInRegisters = 7, kMostInLds = 6;
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a) {
   constexpr int kVec = Io<T>::kVec; // logits of a 16-byte load
   constexpr int kChunk = kThreads * kVec;
   using V = RawVec<T, kVec>;
-  __shared__ SampleLds lds;
+  extern __shared__ __align__(16) unsigned char lds_raw[];
+  SampleLds &lds = *reinterpret_cast<SampleLds *>(lds_raw);
+  V *const lds_held = reinterpret_cast<V *>(lds_raw + sizeof(SampleLds)); // [chunk - kInRegisters][thread]
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int64_t row = blockIdx.x;
   const int vocab = a.vocab;
   const T *const logits = static_cast<const T *>(a.logits) + row * a.row_stride;
-  // Rows of an odd number of logits begin anywhere: loads are 16-byte aligned, and
-  // the row begins `lead` logits into the first.
+  // Rows of an odd number of logits begin anywhere. They are read in the aligned
+  // 16-byte pieces that hold any of them: the row begins `lead` logits into the first
+  // piece (the logits beside the row's in its first and last piece are masked).
   const int lead = (int)((reinterpret_cast<uintptr_t>(logits) & 15u) / sizeof(T));
-  const int chunks = (vocab + lead + kChunk - 1) / kChunk;
-  // index of the first logit of this thread's vector of chunk c (may be negative)
-  auto first_of = [&](int c) __attribute__((always_inline)) { return c * kChunk + tid * kVec - lead; };
-  auto load = [&](int c) __attribute__((always_inline)) {
-    V v;
-    const int i0 = first_of(c);
-    if (i0 >= 0 && i0 + kVec <= vocab) {
-      v = *reinterpret_cast<const V *>(logits + i0);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        v[e] = i0 + e >= 0 && i0 + e < vocab ? logits[i0 + e] : static_cast<T>(-INFINITY);
-    }
-    return v;
+  const V *const pieces = reinterpret_cast<const V *>(logits - lead);
+  const int last_piece = (vocab + lead - 1) / kVec;
+  const int chunks = last_piece / kThreads + 1;
+  const T kNothing = static_cast<T>(-INFINITY);
+  bool infinite = false; // the largest logit is +inf: only those count, as zeros among -inf
+  // index of the first logit of the vector that thread `t` of the block holds of chunk c (may be negative)
+  auto first_of = [&](int c, int t) __attribute__((always_inline)) { return c * kChunk + t * kVec - lead; };
+  auto load_raw = [&](int c, int t) __attribute__((always_inline)) {
+    const int piece = c * kThreads + t;
+    return pieces[piece < last_piece ? piece : last_piece]; // (no branch: the loads of a thread are issued together)
   };
-  // f(chunk, vector) for every vector of the row
-  auto for_chunks = [&](auto &&f) __attribute__((always_inline)) {
-#pragma unroll 1
-    for (int c = 0; c < chunks; ++c) f(c, load(c));
-  };
-  auto value = [](const V &v, int e) __attribute__((always_inline)) {
-    const float x = static_cast<float>(v[e]);
-    return x != x ? -INFINITY : x;
-  };
-
-  // the largest logit, and the smallest finite one
-  float top = -INFINITY, low = INFINITY;
-  for_chunks([&](int, const V &v) __attribute__((always_inline)) {
+  // Beside the row: -inf. NaN becomes -inf, -0 becomes 0 (they are equal logits).
+  auto clean = [&](V &v, int c, int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
-      const float x = value(v, e);
-      top = fmaxf(top, x);
-      low = fminf(low, x == -INFINITY ? INFINITY : x);
+      const float x = static_cast<float>(v[e]) + 0.f;
+      const bool inside = (unsigned)(first_of(c, t) + e) < (unsigned)vocab;
+      v[e] = inside && x == x ? static_cast<T>(x) : kNothing;
     }
+  };
+  auto only_infinite = [&](V &v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) v[e] = static_cast<float>(v[e]) == INFINITY ? static_cast<T>(0.f) : kNothing;
+  };
+  auto load = [&](int c, int t) __attribute__((always_inline)) {
+    V v = load_raw(c, t);
+    clean(v, c, t);
+    if (infinite) only_infinite(v);
+    return v;
+  };
+  V held[kInRegisters];
+  const int in_lds = chunks - kInRegisters < kMostInLds ? chunks - kInRegisters : kMostInLds;
+#pragma unroll
+  for (int c = 0; c < kInRegisters; ++c) held[c] = load_raw(c, tid);
+  if (in_lds > 0) {
+    V more[kMostInLds];
+#pragma unroll
+    for (int c = 0; c < kMostInLds; ++c) more[c] = load_raw(kInRegisters + c, tid);
+#pragma unroll
+    for (int c = 0; c < kMostInLds; ++c)
+      if (c < in_lds) {
+        clean(more[c], kInRegisters + c, tid);
+        lds_held[c * kThreads + tid] = more[c];
+      }
+  }
+#pragma unroll
+  for (int c = 0; c < kInRegisters; ++c) clean(held[c], c, tid);
+  lds.table[tid] = table_entry(tid); // (as many entries as threads)
+  // f(chunk, vector) for every vector of this thread. The empty statement "changes"
+  // the vector: without it the compiler works out ahead, for all chunks at once, what
+  // several passes have in common (conversions, whole masses, indices), and spills it.
+  int at_tid = tid; // the thread, for the indices of the vector being visited
+  auto for_chunks = [&](auto &&f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < kInRegisters; ++c)
+      if (c < chunks) {
+        u32x4_t w = __builtin_bit_cast(u32x4_t, held[c]);
+        at_tid = tid;
+        asm volatile("" : "+v"(w), "+v"(at_tid));
+        f(c, __builtin_bit_cast(V, w));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    at_tid = tid;
+#pragma unroll 1
+    for (int c = kInRegisters; c < chunks; ++c) {
+      V v;
+      if (c < kInRegisters + kMostInLds) v = lds_held[(c - kInRegisters) * kThreads + tid];
+      else v = load(c, tid);
+      f(c, v);
+    }
+  };
+  // the same, all of it read again (for searches that hardly ever run: little code)
+  auto for_chunks_again = [&](auto &&f) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) f(c, load(c, tid));
+  };
+
+  // the largest logit of the thread, then of the row
+  float mine = -INFINITY;
+  for_chunks([&](int, const V &v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) mine = fmaxf(mine, static_cast<float>(v[e]));
   });
-  top = wave_allreduce(top, OpMax());
-  low = -wave_allreduce(-low, OpMax());
+  float top = wave_allreduce(mine, OpMax());
+  float low = -wave_allreduce(mine == -INFINITY ? -INFINITY : -mine, OpMax()); // smallest finite maximum
   if (lane == 0) lds.wave_max[wave] = top, lds.wave_min[wave] = low;
   __syncthreads();
 #pragma unroll
@@ -208,205 +315,513 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a) {
     }
     return;
   }
+  if (top == INFINITY) {
+    infinite = true;
+    mine = mine == INFINITY ? 0.f : -INFINITY;
+    top = low = 0.f;
+#pragma unroll
+    for (int c = 0; c < kInRegisters; ++c) only_infinite(held[c]);
+    for (int c = 0; c < in_lds; ++c) only_infinite(lds_held[c * kThreads + tid]);
+  }
 
   const double temperature = a.temperature.at(row);
-  const bool greedy = !(temperature > 0.0); // the first of the largest
-  const double per_unit = greedy ? 0.0 : 1.4426950408889634074 / temperature;
-  // mass of a logit, relative to the largest one's, and as a whole number of 2^-S
-  auto mass_of = [&](float x) __attribute__((always_inline)) -> double {
-    if (x == top) return 1.0; // (also where both are infinite)
-    return greedy ? 0.0 : exp2_of(((double)x - (double)top) * per_unit);
+  const double k_setting = a.top_k.at(row);
+  if (!(temperature > 0.0) || k_setting == 1.0) { // the first of the largest
+    if (tid == 0) lds.found_at = vocab;
+    __syncthreads();
+    if (mine == top)
+      for_chunks_again([&](int c, const V &v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (static_cast<float>(v[e]) == top) atomicMin(&lds.found_at, first_of(c, tid) + e);
+      });
+    __syncthreads();
+    if (tid == 0) {
+      a.tokens[row] = lds.found_at;
+      if (a.logprobs) a.logprobs[row] = 0.f;
+    }
+    return;
+  }
+
+  // Mass of a logit relative to the largest one's, as a whole number of 2^-S: with
+  // y = (x - top) * log2(e) / temperature = n / 1024 + r, |r| <= 2^-11, it is 2^(n / 1024)
+  // from the table times the series of 2^r = e^(r ln 2) to the third power (the next
+  // term is below 2^-50). The result times 2^S is below 2^52: adding 2^52 leaves the
+  // rounded whole number in the low bits.
+  const double per_unit = 1.4426950408889634074 / temperature;
+  auto units_of = [&](float x) __attribute__((always_inline)) -> u64 {
+    const double y = fmax(((double)x - (double)top) * per_unit, -1200.0); // (nothing from 2^-1075 down)
+    const double t = __builtin_fma(y, (double)kTable, 6755399441055744.0); // 1.5 * 2^52: the rounded n in the low bits
+    const int n = (int)(uint32_t)__builtin_bit_cast(u64, t);
+    const double r = __builtin_fma(t - 6755399441055744.0, -1.0 / kTable, y);
+    constexpr double kLn2 = 0.69314718055994530942;
+    double p = __builtin_fma(r, kLn2 * kLn2 * kLn2 / 6.0, kLn2 * kLn2 / 2.0);
+    p = __builtin_fma(p, r, kLn2);
+    p = __builtin_fma(p, r, 1.0);
+    const double m = __builtin_ldexp(p * lds.table[n & (kTable - 1)], (n >> 10) + a.mass_bits);
+    return __builtin_bit_cast(u64, m + 4503599627370496.0) & 0xfffffffffffffull;
   };
-  const double unit = __builtin_ldexp(1.0, a.mass_bits);
-  auto units_of = [&](double mass) __attribute__((always_inline)) -> u64 {
-    // (below 2^52: adding 2^52 leaves the rounded whole number in the low bits)
-    const double shifted = __builtin_fma(mass, unit, 4503599627370496.0);
-    return __builtin_bit_cast(u64, shifted) & 0xfffffffffffffull;
+  // Steps of the distance to the largest logit, falling as x rises.
+  auto step_of = [&](float x, float per_step) __attribute__((always_inline)) -> int {
+    return (int)fminf((top - x) * per_step, (float)(kBins - 1));
   };
 
-  // Where, along the order, the running weight reaches `target`: the key of the
-  // logit, and the weight that is missing there. `weight(x)` is the whole-number
-  // weight of a logit, 0 for those not to be counted.
-  const float span = top - low;
-  const float per_step = span > 0.f && span < 3.0e38f ? (float)(kBins - 1) / span : 0.f;
-  auto step_of = [&](float x) __attribute__((always_inline)) -> int { // falls as x rises
-    return x == top ? 0 : (int)fminf((top - x) * per_step, (float)(kBins - 1));
+  // The kept front of the order: logits above `cut`, and those equal to it with an
+  // index up to `cut_index`; of those the ones not below `floor_x` (min-p).
+  float cut = -INFINITY, floor_x = -INFINITY;
+  int cut_index = -1;
+  bool cutting = false; // (there is a cut at all)
+  auto in_front = [&](float x, int index) __attribute__((always_inline)) {
+    return x > cut || (x == cut && index <= cut_index);
   };
-  auto select = [&](auto &&weight, u64 target, uint32_t &key, u64 &missing) __attribute__((always_inline)) {
-    for (int b = tid; b < kBins; b += kThreads) lds.bins[b] = 0;
+  const double min_mass = a.min_p.at(row);
+  if (min_mass > 0.0) {
+    // mass >= min_p where the logit reaches top + temperature * ln(min_p); the largest always stays
+    const double least = (double)top + (min_mass < 1.0 ? log(min_mass) * temperature : 0.0);
+    floor_x = (float)least;
+    if ((double)floor_x < least) floor_x = key_value(order_key(floor_x) + 1);
+  }
+  const double p_setting = a.top_p.at(row) < 1.0 ? fmax(a.top_p.at(row), 0.0) : 1.0; // (NaN: everything)
+  double u = (double)a.uniforms[row];
+  u = u >= 0.0 ? (u < 1.0 ? u : 0.99999994039535522) : 0.0;
+  // the target of top-p among `total` units, and of the draw
+  auto share_of = [&](u64 total) __attribute__((always_inline)) -> u64 {
+    const double wanted = __builtin_ceil(p_setting * (double)total);
+    const u64 target = wanted < 1.0 ? 1 : (u64)wanted;
+    return target > total ? total : target;
+  };
+  auto drawn_of = [&](u64 total) __attribute__((always_inline)) -> u64 {
+    const u64 target = (u64)(u * (double)total);
+    return target < total ? target : total - 1;
+  };
+  auto finish = [&](int token, float x, u64 total) __attribute__((always_inline)) { // (one thread)
+    a.tokens[row] = token;
+    if (a.logprobs)
+      a.logprobs[row] = (float)(((double)x - (double)top) / temperature - log(__builtin_ldexp((double)total, -a.mass_bits)));
+  };
+
+  auto clear_bins = [&](u64 *bins) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < kBinsEach; ++b) bins[tid + b * kThreads] = 0;
     __syncthreads();
-    for_chunks([&](int, const V &v) __attribute__((always_inline)) {
+  };
+  // f(entry) for this thread's share of the list
+  auto for_listed = [&](auto &&f) __attribute__((always_inline)) {
+    const int n = lds.listed;
+#pragma unroll 1
+    for (int i = tid; i < n; i += kThreads) {
+      const u64 e = lds.list[i];
+      f(entry_logit(e), entry_index(e));
+    }
+  };
+  auto all_again = [&](auto &&f) __attribute__((always_inline)) {
+    for_chunks_again([&](int c, const V &v) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        const float x = value(v, e);
-        const u64 w = weight(x);
-        if (w) atomicAdd(&lds.bins[step_of(x)], w);
+        const float x = static_cast<float>(v[e]);
+        if (x != -INFINITY) f(x, first_of(c, tid) + e);
       }
     });
+  };
+  auto append = [&](float x, int index) __attribute__((always_inline)) {
+    const int at = atomicAdd(&lds.listed, 1);
+    if (at < kListed) lds.list[at] = list_entry(x, index);
+  };
+  auto start_list = [&]() __attribute__((always_inline)) {
+    if (tid == 0) lds.listed = 0;
     __syncthreads();
-    int step;
-    u64 before;
-    find_bin(lds, kBins, target, step, before);
-    target -= before;
-    // inside the step: the bits of the key from the top, larger keys first
-    uint32_t prefix = 0;
+  };
+  // Up to kRanked listed entries into lds.ranked, in order: four threads (two where
+  // there are more than a quarter of the block) count the entries before one.
+  auto rank_list = [&]() __attribute__((always_inline)) {
+    const int n = lds.listed, share = n <= kThreads / 4 ? 2 : 1, i = tid >> share;
+    if (i < n) {
+      const u64 e = lds.list[i];
+      const int part = tid & ((1 << share) - 1);
+      int before = 0;
+#pragma unroll 8
+      for (int j = part; j < n; j += 1 << share) before += lds.list[j] > e ? 1 : 0;
+      before += __builtin_amdgcn_update_dpp(0, before, 0xB1, 0xf, 0xf, true); // (threads of an entry are neighbours)
+      if (share == 2) before += __builtin_amdgcn_update_dpp(0, before, 0x4E, 0xf, 0xf, true);
+      if (part == 0) lds.ranked[before] = e;
+    }
+    __syncthreads();
+  };
+  constexpr int kRankedEach = kRanked / kWave; // ranks a lane of one wave takes, one behind the other
+
+  // Among the logits that `each` visits: the key at which the running weight reaches
+  // `target`, what is missing there, and the weight of all logits with that key.
+  struct Border {
+    uint32_t key;
+    u64 missing, value;
+  };
+  auto by_bits = [&](auto &&each, auto &&weight, u64 target) __attribute__((always_inline)) {
+    Border r;
+    r.key = 0;
     int bits = 0;
 #pragma unroll 1
     for (int level = 0; level < 3; ++level) {
       const int take = level == 2 ? 10 : 11, shift = 32 - bits - take;
-      for (int b = tid; b < kBins; b += kThreads) lds.bins[b] = 0;
-      __syncthreads();
-      for_chunks([&](int, const V &v) __attribute__((always_inline)) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float x = value(v, e);
-          if (x == -INFINITY || step_of(x) != step) continue;
-          const uint32_t k = order_key(x);
-          if (bits && (k >> (32 - bits)) != prefix) continue;
-          const u64 w = weight(x);
-          if (w) atomicAdd(&lds.bins[((1u << take) - 1) - ((k >> shift) & ((1u << take) - 1))], w);
-        }
+      const uint32_t mask = (1u << take) - 1;
+      clear_bins(lds.bins);
+      each([&](float x, int index) __attribute__((always_inline)) {
+        const uint32_t k = order_key(x);
+        if (bits && (k >> (32 - bits)) != r.key) return;
+        const u64 w = weight(x, index);
+        if (w) atomicAdd(&lds.bins[mask - ((k >> shift) & mask)], w);
       });
       __syncthreads();
-      int bin;
-      find_bin(lds, 1 << take, target, bin, before);
-      target -= before;
-      prefix = prefix << take | (((1u << take) - 1) - (uint32_t)bin);
+      const Found f = find_bin(lds, lds.bins, scan_bins(lds, lds.bins), target);
+      target -= f.before;
+      r.key = r.key << take | (mask - (uint32_t)f.at);
+      r.value = f.value;
       bits += take;
     }
-    key = prefix;
-    missing = target;
+    r.missing = target;
+    return r;
   };
-  // Sum of a weight over the row.
-  auto total_of = [&](auto &&weight) __attribute__((always_inline)) -> u64 {
-    u64 sum = 0;
-    for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
+  // Inside segment `f` of the row (the 64 vectors that one wave holds of a chunk): the
+  // index at which the running weight exceeds `target`. Every thread gets it.
+  auto inside_segment = [&](const Found &f, auto &&weight, u64 target) __attribute__((always_inline)) -> int {
+    if (wave == 0) {
+      const int c = f.at / kWaves, t = f.at % kWaves * kWave + lane;
+      const V v = load(c, t);
+      u64 w[kVec], sum = 0;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum += weight(value(v, e), first_of(c) + e);
-    });
-    sum = wave_sum_u64(sum);
-    __syncthreads();
-    if (lane == 0) lds.wave_sums[wave] = sum;
-    __syncthreads();
-    sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += lds.wave_sums[w];
-    __syncthreads();
-    return sum;
-  };
-  // The first index, in index order, at which the running weight exceeds `target`.
-  auto index_past = [&](auto &&weight, u64 target, double &mass) __attribute__((always_inline)) -> int {
-    u64 run = 0; // weight before the chunk
-    int answer = -1;
-    auto one = [&](int c, const V &v) __attribute__((always_inline)) {
-      if (answer >= 0) return;
-      u64 w[kVec], mine = 0;
+      for (int e = 0; e < kVec; ++e) sum += w[e] = weight(static_cast<float>(v[e]), first_of(c, t) + e);
+      u64 at = f.before + wave_scan_u64(sum, lane) - sum;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        w[e] = weight(value(v, e), first_of(c) + e);
-        mine += w[e];
+        if (at <= target && at + w[e] > target) lds.found_at = first_of(c, t) + e; // exactly one
+        at += w[e];
       }
-      const u64 upto = wave_scan_u64(mine, lane);
-      if (lane == kWave - 1) lds.wave_sums[wave] = upto;
-      __syncthreads();
-      u64 before = run, all = 0;
+    }
+    __syncthreads();
+    const int index = lds.found_at;
+    __syncthreads();
+    return index;
+  };
+  // The index of the `ties`-th of the logits equal to x that are in the front.
+  auto index_of_tie = [&](float x, u64 ties) __attribute__((always_inline)) -> int {
+    auto is_tie = [&](float y, int i) __attribute__((always_inline)) -> u64 { return y == x && in_front(y, i) ? 1 : 0; };
+    clear_bins(lds.bins);
+    for_chunks_again([&](int c, const V &v) __attribute__((always_inline)) {
+      u64 sum = 0;
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
-        if (i < wave) before += lds.wave_sums[i];
-        all += lds.wave_sums[i];
+      for (int e = 0; e < kVec; ++e) sum += is_tie(static_cast<float>(v[e]), first_of(c, tid) + e);
+      sum = wave_sum_u64(sum);
+      if (lane == 0) lds.bins[c * kWaves + wave] = sum;
+    });
+    __syncthreads();
+    const Found f = find_bin(lds, lds.bins, scan_bins(lds, lds.bins), ties);
+    return inside_segment(f, is_tie, ties - 1);
+  };
+  // The front now ends at b.key, of whose logits the first ceil(b.missing / each) are in.
+  auto set_cut = [&](const Border &b, u64 each) __attribute__((always_inline)) {
+    const u64 ties = (b.missing + each - 1) / each;
+    const float x = key_value(b.key);
+    const int index = ties < b.value / each ? index_of_tie(x, ties) : vocab;
+    cut = x;
+    cut_index = index;
+    cutting = true;
+  };
+  auto one_each = [](float, int) __attribute__((always_inline)) -> u64 { return 1; };
+  // The listed entry at which the running weight reaches `target`: entries are
+  // distinct, so their 64 bits, eleven at a time from the top, lead to one (of the
+  // index 19 bits can differ).
+  auto entry_border = [&](auto &&weight, u64 target) __attribute__((always_inline)) -> u64 {
+    u64 prefix = 0;
+    int below = 64; // bits below the prefix
+#pragma unroll 1
+    while (below > 0) {
+      const int take = below == 42 ? 10 : below == 32 ? 13 : below == 8 ? 8 : 11; // 11 11 10 | 13 that are alike, 11, 8
+      if (take == 13) {
+        prefix = prefix << 13 | 0x1fff;
+        below -= 13;
+        continue;
+      }
+      const u64 mask = (1u << take) - 1;
+      clear_bins(lds.bins);
+      const int n = lds.listed;
+#pragma unroll 1
+      for (int i = tid; i < n; i += kThreads) {
+        const u64 e = lds.list[i];
+        if (below < 64 && (e >> below) != prefix) continue;
+        const u64 w = weight(entry_logit(e));
+        if (w) atomicAdd(&lds.bins[mask - ((e >> (below - take)) & mask)], w);
       }
       __syncthreads();
-      if (run + all > target) { // in this chunk (the same for every thread)
-        u64 at = before + upto - mine;
-        if (at <= target && at + mine > target) { // exactly one thread
+      const Found f = find_bin(lds, lds.bins, scan_bins(lds, lds.bins), target);
+      target -= f.before;
+      prefix = prefix << take | (mask - (u64)f.at);
+      below -= take;
+    }
+    return prefix;
+  };
+  auto cut_at = [&](u64 entry) __attribute__((always_inline)) {
+    cut = entry_logit(entry);
+    cut_index = entry_index(entry);
+    cutting = true;
+  };
+
+  if (k_setting > 1.0 && k_setting < (double)vocab) {
+    const u64 k = (u64)k_setting;
+    bool listed = false;
+    if (k <= kThreads) {
+      // the step that the k-th largest of the threads' maxima lies in: the logits up to it are at least k
+      const float per_step = top > low ? fminf((float)(kBins - 1) / (top - low), 1.0e30f) : 0.f;
+      clear_bins(lds.bins);
+      if (mine != -INFINITY) atomicAdd(&lds.bins[step_of(mine, per_step)], (u64)1);
+      __syncthreads();
+      const BinScan s = scan_bins(lds, lds.bins);
+      if (s.total >= k) {
+        const Found f = find_bin(lds, lds.bins, s, k);
+        if (tid == 0) lds.bound = 0xffffffffu;
+        start_list();
+        if (mine != -INFINITY && step_of(mine, per_step) <= f.at) atomicMin(&lds.bound, order_key(mine));
+        __syncthreads();
+        const float bound = key_value(lds.bound); // the smallest of those maxima, of which there are at least k
+        for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
 #pragma unroll
           for (int e = 0; e < kVec; ++e) {
-            if (at <= target && at + w[e] > target) {
-              lds.found_index = first_of(c) + e;
-              lds.found_mass = (double)value(v, e);
-            }
-            at += w[e];
+            const float x = static_cast<float>(v[e]);
+            if (x >= bound) append(x, first_of(c, at_tid) + e);
+          }
+        });
+        __syncthreads();
+        listed = lds.listed <= kListed;
+      }
+      __syncthreads();
+    }
+    if (listed && lds.listed <= kRanked) {
+      // everything that is left fits one wave
+      rank_list();
+      if (wave == 0) {
+        const int n = lds.listed < (int)k ? lds.listed : (int)k;
+        u64 w[kRankedEach], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kRankedEach; ++i) {
+          const int rank = lane * kRankedEach + i;
+          w[i] = rank < n ? units_of(entry_logit(lds.ranked[rank])) : 0;
+          sum += w[i];
+        }
+        const u64 upto = wave_scan_u64(sum, lane);
+        const u64 total = wave_sum_u64(sum);
+        const u64 target = share_of(total);
+        u64 run = upto - sum, kept_sum = 0;
+        int kept = 0;
+#pragma unroll
+        for (int i = 0; i < kRankedEach; ++i) {
+          const int rank = lane * kRankedEach + i;
+          // (every filter keeps a front of the order)
+          if (rank < n && (p_setting >= 1.0 || run < target) && entry_logit(lds.ranked[rank]) >= floor_x) {
+            ++kept;
+            kept_sum += w[i];
+          }
+          run += w[i];
+        }
+        kept_sum = wave_sum_u64(kept_sum);
+        const int all_kept = (int)wave_sum_u64((u64)kept);
+        if (lane == 0) lds.listed = all_kept, lds.found_value = kept_sum;
+      }
+      __syncthreads();
+      // in index order: the threads of an entry sum the kept masses up to its index
+      const int n = lds.listed, share = n <= kThreads / 4 ? 2 : 1, i = tid >> share, part = tid & ((1 << share) - 1);
+      const u64 total = lds.found_value, target = drawn_of(total);
+      u64 *const units = lds.bins; // (nothing else is in the bins now)
+      if (tid < n) units[tid] = units_of(entry_logit(lds.ranked[tid]));
+      __syncthreads();
+      if (i < n) {
+        const int index = entry_index(lds.ranked[i]);
+        u64 before = 0;
+#pragma unroll 8
+        for (int j = part; j < n; j += 1 << share) before += entry_index(lds.ranked[j]) < index ? units[j] : 0;
+        before += dpp_u64<0xB1>(before);
+        if (share == 2) before += dpp_u64<0x4E>(before);
+        if (part == 0 && before <= target && before + units[i] > target)
+          finish(index, entry_logit(lds.ranked[i]), total);
+      }
+      return;
+    }
+    if (listed) {
+      cut_at(entry_border([](float) __attribute__((always_inline)) -> u64 { return 1; }, k));
+    } else { // every logit, where there are more than k of them to count
+      clear_bins(lds.bins);
+      u64 count = 0;
+      all_again([&](float, int) __attribute__((always_inline)) { ++count; });
+      count = wave_sum_u64(count);
+      if (lane == 0) lds.bins[wave] = count;
+      __syncthreads();
+      const BinScan s = scan_bins(lds, lds.bins);
+      __syncthreads();
+      if (s.total > k) set_cut(by_bits(all_again, one_each, k), 1);
+    }
+  }
+
+  // Top-p over what is left: the hint, then the exact pass. Logits above `sure_x` are
+  // surely kept, those from `window_x` up to it are listed.
+  float sure_x = -INFINITY, window_x = INFINITY;
+  bool window = false;
+  if (p_setting < 1.0) {
+    // 2048 steps over 2^26 of mass; what is smaller is in the last one and counts as nothing
+    constexpr float kPerHalving = (float)(kBins - 1) / 26.0f;
+    const float per_step = (float)fmin(kPerHalving * per_unit, 1.0e30);
+    uint32_t *const counts = reinterpret_cast<uint32_t *>(lds.segments);
+    clear_bins(lds.segments);
+    for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const float x = static_cast<float>(v[e]);
+        const int step = step_of(x, per_step);
+        if (step < kBins - 1 && (!cutting || in_front(x, first_of(c, at_tid) + e))) atomicAdd(&counts[step], 1u);
+      }
+    });
+    __syncthreads();
+    // (2^40 to the largest mass, each taken at the middle of its step)
+#pragma unroll
+    for (int i = 0; i < kBinsEach; ++i) {
+      const int b = tid_bin(i);
+      lds.bins[b] = (u64)((float)counts[b] * __builtin_amdgcn_exp2f(40.0f - ((float)b + 0.5f) / kPerHalving));
+    }
+    __syncthreads();
+    const BinScan s = scan_bins(lds, lds.bins);
+    // Every mass is off by at most a factor 1 +- 0.0044, so a share p by at most 0.0088 p (1 - p).
+    const u64 target = share_of(s.total);
+    const u64 slack = (u64)((double)s.total * (0.009 * p_setting * (1.0 - p_setting) + 1.0e-5));
+    const Found from = find_bin(lds, lds.bins, s, target > slack ? target - slack : 1);
+    const Found to = find_bin(lds, lds.bins, s, target + slack < s.total ? target + slack : s.total);
+    sure_x = from.at == 0 ? INFINITY : top - ((float)from.at - 0.25f) / per_step;
+    window_x = top - ((float)to.at + 1.25f) / per_step;
+    window = true;
+  }
+  // Where min-p cuts above the window, nothing in the window stays: the logits that
+  // min-p keeps are the answer if top-p's share is not reached before the last of them.
+  const bool by_floor = window && floor_x > sure_x;
+  if (by_floor) window_x = INFINITY;
+  if (by_floor || !window) sure_x = next_below(floor_x);
+  auto kept_units = [&](float x, int i) __attribute__((always_inline)) -> u64 {
+    return in_front(x, i) && x >= floor_x ? units_of(x) : 0;
+  };
+  while (true) {
+    start_list();
+    clear_bins(lds.segments);
+    u64 all = 0; // what top-p is a share of
+    for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
+      u64 kept = 0;
+#pragma unroll
+      for (int e0 = 0; e0 < kVec; e0 += 4) { // (four at a time: the masses of eight do not fit the registers)
+        u64 w[4];
+        bool near = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = units_of(static_cast<float>(v[e0 + e]));
+        if (cutting)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = in_front(static_cast<float>(v[e0 + e]), first_of(c, at_tid) + e0 + e) ? w[e] : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = static_cast<float>(v[e0 + e]);
+          all += w[e];
+          kept += x > sure_x ? w[e] : 0;
+          near |= x >= window_x && x <= sure_x;
+        }
+        if (near)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = static_cast<float>(v[e0 + e]);
+            if (x >= window_x && x <= sure_x && w[e]) append(x, first_of(c, at_tid) + e0 + e);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      kept = wave_sum_u64(kept);
+      if (lane == 0) lds.segments[c * kWaves + wave] = kept;
+    });
+    if (!window) break;
+    all = wave_sum_u64(all);
+    if (lane == 0) lds.bins[wave] = all;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all += lds.bins[w];
+    const u64 above = scan_bins(lds, lds.segments).total;
+    __syncthreads();
+    const u64 target = share_of(all);
+    const int n = lds.listed;
+    u64 listed_units = 0;
+    if (by_floor && above <= target) break;
+    if (!by_floor && n <= kListed) {
+      for_listed([&](float x, int) __attribute__((always_inline)) { listed_units += units_of(x); });
+      listed_units = wave_sum_u64(listed_units);
+      if (lane == 0) lds.bins[wave] = listed_units;
+      __syncthreads();
+      listed_units = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) listed_units += lds.bins[w];
+      __syncthreads();
+    }
+    if (!by_floor && target > above && target <= above + listed_units) {
+      // the border is among the listed ones; those in front of it join their segments
+      if (n <= kRanked) {
+        rank_list();
+        if (wave == 0) {
+          u64 w[kRankedEach], sum = 0;
+#pragma unroll
+          for (int i = 0; i < kRankedEach; ++i) {
+            const int rank = lane * kRankedEach + i;
+            sum += w[i] = rank < n ? units_of(entry_logit(lds.ranked[rank])) : 0;
+          }
+          u64 run = above + wave_scan_u64(sum, lane) - sum;
+#pragma unroll
+          for (int i = 0; i < kRankedEach; ++i) {
+            if (run < target && run + w[i] >= target) lds.found_at = lane * kRankedEach + i; // exactly one
+            run += w[i];
           }
         }
         __syncthreads();
-        answer = lds.found_index;
-        mass = lds.found_mass;
+        cut_at(lds.ranked[lds.found_at]);
+      } else {
+        cut_at(entry_border(units_of, target - above));
       }
-      run += all;
-    };
-    for_chunks(one);
-    return answer;
-  };
-
-  // the kept front of the order: logits with a key above `cut_key`, and those with
-  // that key and an index up to `cut_index`
-  uint32_t cut_key = 0;
-  int cut_index = vocab;
-  auto in_front = [&](float x, int index) __attribute__((always_inline)) {
-    const uint32_t k = order_key(x);
-    return x != -INFINITY && (k > cut_key || (k == cut_key && index <= cut_index));
-  };
-  auto set_cut = [&](uint32_t key, u64 ties) __attribute__((always_inline)) { // the first `ties` of the logits with this key
-    cut_key = key;
-    double unused;
-    cut_index = index_past([&](float x, int) __attribute__((always_inline)) -> u64 { return order_key(x) == key ? 1 : 0; },
-                           ties - 1, unused);
-  };
-  const double k_setting = a.top_k.at(row);
-  if (greedy || (k_setting > 0.0 && k_setting < (double)vocab)) {
-    const u64 k = greedy ? 1 : (u64)k_setting;
-    // (with fewer finite logits than k there is nothing to cut)
-    const u64 finite = total_of([&](float x, int) __attribute__((always_inline)) -> u64 { return x == -INFINITY ? 0 : 1; });
-    if (finite > k) {
-      uint32_t key;
-      u64 ties;
-      select([&](float x) __attribute__((always_inline)) -> u64 { return x == -INFINITY ? 0 : 1; }, k, key, ties);
-      set_cut(key, ties);
+      for_listed([&](float x, int i) __attribute__((always_inline)) {
+        const u64 w = kept_units(x, i);
+        if (w) atomicAdd(&lds.segments[(i + lead) / kChunk * kWaves + (i + lead) % kChunk / (kWave * kVec)], w);
+      });
+      break;
     }
+    // the hint was off, or its step too full: the exact search, and the pass again without a window
+    const Border b = by_bits(all_again, [&](float x, int i) __attribute__((always_inline)) -> u64 {
+      return in_front(x, i) ? units_of(x) : 0;
+    }, target);
+    set_cut(b, units_of(key_value(b.key)));
+    window = false;
+    window_x = INFINITY;
+    sure_x = next_below(floor_x);
   }
-  const double p_setting = greedy ? 1.0 : a.top_p.at(row);
-  if (p_setting < 1.0) {
-    const u64 all = total_of([&](float x, int i) __attribute__((always_inline)) -> u64 {
-      return in_front(x, i) ? units_of(mass_of(x)) : 0;
-    });
-    const double wanted = __builtin_ceil((p_setting > 0.0 ? p_setting : 0.0) * (double)all);
-    u64 target = wanted < 1.0 ? 1 : (u64)wanted;
-    if (target > all) target = all;
-    const uint32_t floor_key = cut_key;
-    uint32_t key;
-    u64 missing;
-    select([&](float x) __attribute__((always_inline)) -> u64 {
-      return x != -INFINITY && order_key(x) >= floor_key ? units_of(mass_of(x)) : 0;
-    }, target, key, missing);
-    const float cut = __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
-    const u64 each = units_of(mass_of(cut));
-    const u64 ties = (missing + each - 1) / each;
-    set_cut(key, ties);
-  }
-  const double min_mass = greedy ? 0.0 : fmin(a.min_p.at(row), 1.0); // (the largest always stays)
-  auto kept_units = [&](float x, int i) __attribute__((always_inline)) -> u64 {
-    if (!in_front(x, i)) return 0;
-    const double mass = mass_of(x);
-    return mass >= min_mass ? units_of(mass) : 0;
-  };
-  const u64 all = total_of(kept_units);
-  double u = (double)a.uniforms[row];
-  u = u >= 0.0 ? (u < 1.0 ? u : 0.99999994039535522) : 0.0;
-  u64 target = (u64)(u * (double)all);
-  if (target >= all) target = all - 1;
-  double logit = 0.0;
-  int token = index_past(kept_units, target, logit);
+  __syncthreads();
+  const BinScan s = scan_bins(lds, lds.segments);
+  const u64 target = drawn_of(s.total);
+  const Found f = find_bin(lds, lds.segments, s, target + 1);
+  const int token = inside_segment(f, kept_units, target);
   if (tid == 0) {
-    a.tokens[row] = token;
-    if (a.logprobs)
-      a.logprobs[row] = (float)(((float)logit == top ? 0.0 : (logit - (double)top) * (greedy ? 0.0 : 1.0 / temperature)) -
-                                log((double)all / unit));
+    const float x = static_cast<float>(logits[token]) + 0.f;
+    finish(token, infinite ? 0.f : x, s.total);
   }
 }
 
+// Logits a row may have: its segments have to fit the bins.
+constexpr int64_t kMaxVocab = 500000;
+static_assert(kMaxVocab + 8 <= (int64_t)kBins / kWaves * kThreads * 4, "a bin per segment");
+
 template <typename T>
 int launch_sample(const SampleArgs &a, int64_t rows, hipStream_t stream) {
-  sample_kernel<T><<<dim3((unsigned)rows), dim3(kThreads), 0, stream>>>(a);
+  constexpr int kChunk = kThreads * Io<T>::kVec;
+  const int chunks = (a.vocab + Io<T>::kVec - 1 + kChunk - 1) / kChunk;
+  const int in_lds = chunks <= kInRegisters ? 0 : chunks - kInRegisters < kMostInLds ? chunks - kInRegisters : kMostInLds;
+  const unsigned bytes = (unsigned)(sizeof(SampleLds) + (size_t)in_lds * kThreads * 16);
+  constexpr unsigned kMostBytes = (unsigned)(sizeof(SampleLds) + (size_t)kMostInLds * kThreads * 16);
+  const int s = raise_lds_limit(reinterpret_cast<const void *>(sample_kernel<T>), kMostBytes, "oslo_sample");
+  if (s != OSLO_OK) return s;
+  sample_kernel<T><<<dim3((unsigned)rows), dim3(kThreads), bytes, stream>>>(a);
   return check_launch("sample");
 }
 
@@ -427,7 +842,7 @@ extern "C" int oslo_sample(int64_t *tokens, float *logprobs, const void *logits,
   if (!min_ps && !(min_p >= 0.0 && min_p <= 1.0)) return fail(OSLO_E_BAD_ARG, "oslo_sample: min_p must be in [0, 1]");
   if (rows == 0) return OSLO_OK;
   if (vocab == 0) return fail(OSLO_E_BAD_ARG, "oslo_sample: no logits to draw from");
-  if (vocab > (int64_t)1 << 24) return fail(OSLO_E_UNSUPPORTED, "oslo_sample: more than 2^24 logits a row");
+  if (vocab > kMaxVocab) return fail(OSLO_E_UNSUPPORTED, "oslo_sample: more than %lld logits a row", (long long)kMaxVocab);
   if (rows > (int64_t)0x7fffffff) return fail(OSLO_E_UNSUPPORTED, "oslo_sample: too many rows for one launch");
   if (!tokens || !logits || !uniforms) return fail(OSLO_E_BAD_ARG, "oslo_sample: null pointer");
   SampleArgs a;
