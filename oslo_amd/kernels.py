@@ -28,11 +28,15 @@ def _require(cond, msg):
 
 
 def _dtype_code(t, what):
-    _require(t.dtype in _DTYPE, f"{what}: only fp16, bf16 and fp32 are supported, got {t.dtype}")
-    return _DTYPE[t.dtype]
+    code = _DTYPE.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{what}: only fp16, bf16 and fp32 are supported, got {t.dtype}")
+    return code
 
 
 def _device_tensor(t, what, like=None):
+    if isinstance(t, torch.Tensor) and t.is_cuda and (like is None or t.device == like.device):
+        return  # (the messages below are only put together where one is needed)
     _require(isinstance(t, torch.Tensor), f"{what}: expected a tensor")
     _require(t.is_cuda, f"{what}: expected a tensor on a ROCm device, got {t.device} "
                         "(this library has no CPU path)")
@@ -46,7 +50,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 def _stream(t):
     """torch's current stream on t's device, as the library's stream argument."""
     if _raw_stream is not None:
-        return ctypes.c_void_p(_raw_stream(t.device.index))
+        return _raw_stream(t.device.index)
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
@@ -70,7 +74,7 @@ def _on_device(t):
 
 
 def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+    return t.data_ptr() if t is not None else None
 
 
 # ---------------------------------------------------------------------------
@@ -722,10 +726,16 @@ def attention_prefill_backward(grad_out, query, key, value, out, lse, scale, pad
 # sequences of different lengths: packed rows, the paged cache, sampling
 # ---------------------------------------------------------------------------
 
+_HALVES = (torch.float16, torch.bfloat16)
+_Strides = {n: ctypes.c_int64 * n for n in (2, 4, 8, 16)}
+
+
 def _packed_strided(t):
-    """t [T, heads, D] as the packed attention can read it; a copy if not."""
-    ok = t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.stride(0) >= t.shape[2] \
-        and t.data_ptr() % 16 == 0
+    """t [T, heads, D] as the kernels over packed tokens can read it; a copy if not."""
+    if t.is_contiguous():
+        return t if t.data_ptr() % 16 == 0 else t.clone()
+    st, sh, sd = t.stride()
+    ok = sd == 1 and st % 8 == 0 and sh % 8 == 0 and st >= t.shape[2] and t.data_ptr() % 16 == 0
     return t if ok else t.contiguous()
 
 
@@ -734,25 +744,33 @@ def _packed_args(query, key, value, packed):
     _device_tensor(key, "key", query)
     _device_tensor(value, "value", query)
     code = _dtype_code(query, "query")
-    _require(query.dtype in (torch.float16, torch.bfloat16), "attention_packed: fp16 or bf16 tensors")
-    _require(query.dim() == 3 and key.dim() == 3 and key.shape == value.shape,
-             "query must be [tokens, heads, D], key and value [tokens, key/value heads, D]")
-    _require(key.dtype == query.dtype and value.dtype == query.dtype, "query, key and value differ in dtype")
+    if query.dtype not in _HALVES:
+        raise RuntimeError("attention_packed: fp16 or bf16 tensors")
+    if query.dim() != 3 or key.dim() != 3 or key.shape != value.shape:
+        raise RuntimeError("query must be [tokens, heads, D], key and value [tokens, key/value heads, D]")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise RuntimeError("query, key and value differ in dtype")
     t, h, d = query.shape
-    hkv = key.shape[1]
-    _require(key.shape[0] == t and key.shape[2] == d, "query, key and value differ in tokens or features")
-    _require(hkv > 0 and h % hkv == 0 if h else True, f"{h} query heads do not share {hkv} key/value heads evenly")
-    _require(d in PREFILL_HEAD_DIMS, f"attention_packed: heads of {d} features (64, 128 or 256 are taken)")
-    _require(packed.total <= t, f"the sequences have {packed.total} tokens, the tensors {t}")
-    _require(packed.blocks.device == query.device, f"the sequences are on {packed.blocks.device}, query on {query.device}")
+    tk, hkv, dk = key.shape
+    if tk != t or dk != d:
+        raise RuntimeError("query, key and value differ in tokens or features")
+    if h and (hkv == 0 or h % hkv):
+        raise RuntimeError(f"{h} query heads do not share {hkv} key/value heads evenly")
+    if d not in PREFILL_HEAD_DIMS:
+        raise RuntimeError(f"attention_packed: heads of {d} features (64, 128 or 256 are taken)")
+    if packed.total > t:
+        raise RuntimeError(f"the sequences have {packed.total} tokens, the tensors {t}")
+    if packed.blocks.device != query.device:
+        raise RuntimeError(f"the sequences are on {packed.blocks.device}, query on {query.device}")
     return code
 
 
-def _token_strides(tensors):
-    strides = (ctypes.c_int64 * (2 * len(tensors)))()
-    for i, t in enumerate(tensors):
-        strides[2 * i], strides[2 * i + 1] = t.stride(1), t.stride(0)
-    return strides
+def _token_strides(*tensors):
+    flat = []
+    for t in tensors:
+        st, sh, _ = t.stride()
+        flat += (sh, st)
+    return _Strides[len(flat)](*flat)
 
 
 def _packed_empty(tokens, heads, d, packed, like):
@@ -771,15 +789,15 @@ def attention_packed_forward(query, key, value, packed, scale, window=0, want_ls
     fp32 [H, T] log2-sum-exp that ``attention_packed_backward`` takes."""
     code = _packed_args(query, key, value, packed)
     t, h, d = query.shape
-    q, k, v = (_packed_strided(x) for x in (query, key, value))
+    q, k, v = _packed_strided(query), _packed_strided(key), _packed_strided(value)
     out = _packed_empty(t, h, d, packed, query)
     lse = torch.empty((h, t), dtype=torch.float32, device=query.device) if want_lse else None
     if packed.total and h:
+        blocks = packed.blocks
         with _on_device(q):
             _lib.check(_lib.load().oslo_attention_packed_fwd(
-                _ptr(out), _ptr(lse), _ptr(q), _ptr(k), _ptr(v), _ptr(packed.blocks[0]), packed.blocks.shape[1],
-                float(scale), t, packed.max_length, h, k.shape[1], d, int(window), _token_strides((q, k, v, out)),
-                code, _stream(q)))
+                out.data_ptr(), _ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), blocks.shape[1],
+                scale, t, packed.max_length, h, k.shape[1], d, window, _token_strides(q, k, v, out), code, _stream(q)))
     return (out, lse) if want_lse else out
 
 
@@ -789,7 +807,8 @@ def attention_packed_backward(grad_out, query, key, value, out, lse, packed, sca
     code = _packed_args(query, key, value, packed)
     for what, x in (("grad_out", grad_out), ("out", out)):
         _device_tensor(x, what, query)
-        _require(x.shape == query.shape and x.dtype == query.dtype, f"{what} must be like query")
+        if x.shape != query.shape or x.dtype != query.dtype:
+            raise RuntimeError(f"{what} must be like query")
     _device_tensor(lse, "lse", query)
     t, h, d = query.shape
     hkv = key.shape[1]
@@ -805,27 +824,29 @@ def attention_packed_backward(grad_out, query, key, value, out, lse, packed, sca
         with _on_device(q):
             _lib.check(lib.oslo_attention_packed_bwd(
                 _ptr(dq), _ptr(dk), _ptr(dv), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(ws),
-                _ptr(packed.blocks[0]), _ptr(packed.blocks[1]), packed.blocks.shape[1], float(scale), t,
-                packed.max_length, h, hkv, d, int(window), _token_strides((q, k, v, o, g, dq, dk, dv)), code,
-                _stream(q)))
+                _ptr(packed.blocks[0]), _ptr(packed.blocks[1]), packed.blocks.shape[1], scale, t,
+                packed.max_length, h, hkv, d, window, _token_strides(q, k, v, o, g, dq, dk, dv), code, _stream(q)))
     return dq, dk, dv
 
 
 def _index_tensor(t, what, like, length):
     _device_tensor(t, what, like)
-    _require(t.dtype == torch.int32 and tuple(t.shape) == (length,), f"{what} must be int32 [{length}]")
-    return t.contiguous()
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != length:
+        raise RuntimeError(f"{what} must be int32 [{length}]")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _cache_args(cache, like, what):
     """What every call over a ``PagedKV`` passes on: its pointers and sizes."""
-    _require(cache.key_pages.device == like.device, f"the cache is on {cache.key_pages.device}, {what} on {like.device}")
-    _require(like.dtype in (torch.float16, torch.bfloat16), f"{what}: fp16 or bf16, got {like.dtype}")
-    _require(cache.quantized or cache.key_pages.dtype == like.dtype,
-             f"{what} is {like.dtype}, the cache {cache.key_pages.dtype}")
-    pages, hkv, page, d = cache.key_pages.shape
-    return (_ptr(cache.key_pages), _ptr(cache.value_pages), _ptr(cache.key_scales), _ptr(cache.value_scales)), \
-        (cache.table.shape[0], cache.table.shape[1], pages), (hkv, page, d)
+    keys = cache.key_pages
+    if keys.device != like.device:
+        raise RuntimeError(f"the cache is on {keys.device}, {what} on {like.device}")
+    if like.dtype not in _HALVES:
+        raise RuntimeError(f"{what}: fp16 or bf16, got {like.dtype}")
+    pointers = (keys.data_ptr(), cache.value_pages.data_ptr(), _ptr(cache.key_scales), _ptr(cache.value_scales))
+    if not cache.quantized and keys.dtype != like.dtype:
+        raise RuntimeError(f"{what} is {like.dtype}, the cache {keys.dtype}")
+    return pointers, (*cache.table.shape, keys.shape[0]), keys.shape[1:]
 
 
 def paged_kv_write(cache, key, value, sequence, position):
@@ -836,15 +857,17 @@ def paged_kv_write(cache, key, value, sequence, position):
     _device_tensor(value, "value", key)
     code = _dtype_code(key, "key")
     pointers, counts, (hkv, page, d) = _cache_args(cache, key, "key")
-    _require(key.dim() == 3 and tuple(key.shape[1:]) == (hkv, d), f"key must be [tokens, {hkv}, {d}]")
-    _require(value.shape == key.shape and value.dtype == key.dtype, "key and value differ in shape or dtype")
+    if key.dim() != 3 or key.shape[1] != hkv or key.shape[2] != d:
+        raise RuntimeError(f"key must be [tokens, {hkv}, {d}]")
+    if value.shape != key.shape or value.dtype != key.dtype:
+        raise RuntimeError("key and value differ in shape or dtype")
     t = key.shape[0]
     sequence, position = _index_tensor(sequence, "sequence", key, t), _index_tensor(position, "position", key, t)
     k, v = _packed_strided(key), _packed_strided(value)
     with _on_device(k):
         _lib.check(_lib.load().oslo_paged_kv_write(
-            *pointers, _ptr(k), _ptr(v), _ptr(sequence), _ptr(position), _ptr(cache.table), t, *counts, hkv, page, d,
-            _token_strides((k, v)), code, _stream(k)))
+            *pointers, k.data_ptr(), v.data_ptr(), sequence.data_ptr(), position.data_ptr(), cache.table.data_ptr(), t,
+            *counts, hkv, page, d, _token_strides(k, v), code, _stream(k)))
 
 
 def paged_kv_read(cache, sequence, position, dtype):
@@ -855,14 +878,14 @@ def paged_kv_read(cache, sequence, position, dtype):
     t = sequence.shape[0]
     sequence, position = (_index_tensor(x, what, cache.key_pages, t) for x, what in
                           ((sequence, "sequence"), (position, "position")))
-    pages, hkv, page, d = cache.key_pages.shape
+    _, hkv, page, d = cache.key_pages.shape
     key, value = (torch.empty((t, hkv, d), dtype=dtype, device=sequence.device) for _ in range(2))
     code = _dtype_code(key, "dtype")
     pointers, counts, _ = _cache_args(cache, key, "dtype")
     with _on_device(key):
         _lib.check(_lib.load().oslo_paged_kv_read(
-            _ptr(key), _ptr(value), *pointers, _ptr(sequence), _ptr(position), _ptr(cache.table), t, *counts, hkv,
-            page, d, code, _stream(key)))
+            key.data_ptr(), value.data_ptr(), *pointers, sequence.data_ptr(), position.data_ptr(),
+            cache.table.data_ptr(), t, *counts, hkv, page, d, code, _stream(key)))
     return key, value
 
 
@@ -873,34 +896,39 @@ def attention_paged_decode_forward(query, cache, lengths, scale, window=0):
     _device_tensor(query, "query")
     code = _dtype_code(query, "query")
     pointers, counts, (hkv, page, d) = _cache_args(cache, query, "query")
-    _require(query.dim() == 3 and query.shape[2] == d, f"query must be [sequences, heads, {d}]")
+    if query.dim() != 3 or query.shape[2] != d:
+        raise RuntimeError(f"query must be [sequences, heads, {d}]")
     b, h, _ = query.shape
-    _require(b == counts[0], f"{b} queries for a table of {counts[0]} sequences")
-    _require(hkv > 0 and h % hkv == 0, f"{h} query heads do not share {hkv} key/value heads evenly")
+    if b != counts[0]:
+        raise RuntimeError(f"{b} queries for a table of {counts[0]} sequences")
+    if hkv == 0 or h % hkv:
+        raise RuntimeError(f"{h} query heads do not share {hkv} key/value heads evenly")
     lengths = _index_tensor(lengths, "lengths", query, b)
     q = query
-    if not (q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0 and q.data_ptr() % 16 == 0):
-        q = q.contiguous()
+    qb, qh, qd = q.stride()
+    if qd != 1 or qb % 8 or qh % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+        qb, qh, _ = q.stride()
     lib = _lib.load()
-    nbytes = lib.oslo_attention_paged_decode_workspace_bytes(b, h, hkv, d, counts[1] * page, int(window))
+    nbytes = lib.oslo_attention_paged_decode_workspace_bytes(b, h, hkv, d, counts[1] * page, window)
     ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
     out = torch.empty((b, h, d), dtype=q.dtype, device=q.device)
-    strides = (ctypes.c_int64 * 2)(q.stride(0), q.stride(1))
     with _on_device(q):
         _lib.check(lib.oslo_attention_paged_decode_fwd(
-            _ptr(out), _ptr(q), *pointers, _ptr(cache.table), _ptr(lengths), _ptr(ws), float(scale), *counts, h, hkv,
-            page, d, int(window), strides, code, _stream(q)))
+            out.data_ptr(), q.data_ptr(), *pointers, cache.table.data_ptr(), lengths.data_ptr(), _ptr(ws), scale,
+            *counts, h, hkv, page, d, window, _Strides[2](qb, qh), code, _stream(q)))
     return out
 
 
 def _row_setting(value, what, dtype, rows, like):
     """(pointer holder, number) of a sampling setting: a tensor of one value per
     row, or a number for all."""
-    if isinstance(value, torch.Tensor):
-        _device_tensor(value, what, like)
-        _require(value.dtype == dtype and tuple(value.shape) == (rows,), f"{what} must be a number or {dtype} [{rows}]")
-        return value.contiguous(), 0
-    return None, value
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    _device_tensor(value, what, like)
+    if value.dtype != dtype or value.dim() != 1 or value.shape[0] != rows:
+        raise RuntimeError(f"{what} must be a number or {dtype} [{rows}]")
+    return value.contiguous(), 0
 
 
 def sample_forward(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -909,22 +937,24 @@ def sample_forward(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=
     number or a device tensor of one value per row (fp32; top_k int32)."""
     _device_tensor(logits, "logits")
     code = _dtype_code(logits, "logits")
-    _require(logits.dim() == 2, "logits must be [rows, vocabulary]")
+    if logits.dim() != 2:
+        raise RuntimeError("logits must be [rows, vocabulary]")
     rows, vocab = logits.shape
     _device_tensor(uniforms, "uniforms", logits)
-    _require(uniforms.dtype == torch.float32 and tuple(uniforms.shape) == (rows,), f"uniforms must be fp32 [{rows}]")
+    if uniforms.dtype != torch.float32 or uniforms.dim() != 1 or uniforms.shape[0] != rows:
+        raise RuntimeError(f"uniforms must be fp32 [{rows}]")
     temperature, temperature_all = _row_setting(temperature, "temperature", torch.float32, rows, logits)
     top_k, top_k_all = _row_setting(top_k, "top_k", torch.int32, rows, logits)
     top_p, top_p_all = _row_setting(top_p, "top_p", torch.float32, rows, logits)
     min_p, min_p_all = _row_setting(min_p, "min_p", torch.float32, rows, logits)
-    x = logits if logits.stride(1) == 1 and (rows <= 1 or logits.stride(0) >= 0) else logits.contiguous()
+    x = logits if logits.stride(1) == 1 else logits.contiguous()
     uniforms = uniforms.contiguous()
     tokens = torch.empty((rows,), dtype=torch.int64, device=x.device)
     logprobs = torch.empty((rows,), dtype=torch.float32, device=x.device)
     with _on_device(x):
         _lib.check(_lib.load().oslo_sample(
-            _ptr(tokens), _ptr(logprobs), _ptr(x), _ptr(uniforms), _ptr(temperature), float(temperature_all),
-            _ptr(top_k), int(top_k_all), _ptr(top_p), float(top_p_all), _ptr(min_p), float(min_p_all), rows, vocab,
+            tokens.data_ptr(), logprobs.data_ptr(), x.data_ptr(), uniforms.data_ptr(), _ptr(temperature),
+            temperature_all, _ptr(top_k), int(top_k_all), _ptr(top_p), top_p_all, _ptr(min_p), min_p_all, rows, vocab,
             x.stride(0), code, _stream(x)))
     return tokens, logprobs
 
