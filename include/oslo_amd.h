@@ -609,7 +609,10 @@ int oslo_attention_packed_fwd(void *out, float *lse, const void *q,
                               oslo_stream_t stream);
 
 /* Bytes of fp32 workspace oslo_attention_packed_bwd needs. */
-size_t oslo_attention_packed_bwd_workspace_bytes(int64_t tokens, int64_t heads);
+size_t oslo_attention_packed_bwd_workspace_bytes(int64_t tokens, int64_t heads,
+                                                 int64_t kv_heads,
+                                                 int64_t head_dim,
+                                                 int64_t split, int64_t parts);
 
 /*
  * Gradients of the packed attention from dout, the inputs, the forward's out and
@@ -617,6 +620,9 @@ size_t oslo_attention_packed_bwd_workspace_bytes(int64_t tokens, int64_t heads);
  * summed over the query heads of a group in fp32, in a fixed order, and rounded
  * once. query_blocks and key_blocks hold the same entries as the forward's
  * `blocks` (most keys first, and most queries left first, run fastest).
+ * The work on the first `split` entries of key_blocks is shared by `parts` blocks
+ * each, which take the heads of a group between them (1 <= parts <= heads /
+ * kv_heads; split 0: none); it changes the order of the fp32 sums, nothing else.
  * strides[16]: head and token strides of q, k, v, out, dout, dq, dk, dv. Rows of
  * no sequence are not written. workspace: 16-byte aligned, contents irrelevant
  * before and after. No output may alias an input. Same bits from run to run.
@@ -627,7 +633,7 @@ int oslo_attention_packed_bwd(void *dq, void *dk, void *dv, const void *dout,
                               const void *out, const float *lse,
                               float *workspace, const int32_t *query_blocks,
                               const int32_t *key_blocks, int64_t num_blocks,
-                              float scale, int64_t tokens, int64_t max_length,
+                              int64_t split, int64_t parts, float scale, int64_t tokens, int64_t max_length,
                               int64_t heads, int64_t kv_heads,
                               int64_t head_dim, int64_t window,
                               const int64_t *strides, int dtype,

@@ -97,7 +97,16 @@ struct BwdArgs {
   unsigned char *tiles;
   int bh0;
   int64_t head_tiles;
-  PackedArgs packed; // the sequences of the PACKED variant
+  // The PACKED variant: the sequences; the forward's output, from which the pass that owns queries works
+  // out delta itself (and leaves it for the passes that own keys); and the entries whose group of
+  // query heads is shared by `parts` blocks (the first `split` of the list: those with most queries),
+  // which leave fp32 sums [entry * parts + part][kv head][dK, dV][128][D] in `partial`.
+  PackedArgs packed;
+  const void *out;
+  Strides3 sout;
+  float *delta_out;
+  float *partial;
+  int split, parts;
 };
 
 // The tile store. P (after dropout) and dS / scale of the 32 queries x 32 keys of
@@ -168,13 +177,30 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
   int64_t start = 0;   // the sequence's first token
   int64_t packed_row = 0; // the (first) query head's row of per-position values
   int64_t stat_step = 0; // from a query head's row to the next head's
+  int group_heads = 1;   // query heads the block walks
+  int64_t part_slot = -1; // of its fp32 sums, if it walks a part of the group only
   if constexpr (PACKED) {
     const unsigned per_entry = kKeysOwn ? (unsigned)a.packed.kv_heads : (unsigned)a.heads;
-    const PackedBlock e = packed_block(a.packed, blockIdx.x / per_entry);
+    const int r = (int)(blockIdx.x % per_entry);
+    unsigned entry = blockIdx.x / per_entry;
+    int first_head = 0; // of the group
+    if constexpr (kKeysOwn) {
+      group_heads = a.packed.group;
+      const unsigned shared = (unsigned)(a.split * a.parts);
+      if (entry < shared) {
+        const int part = (int)(entry % (unsigned)a.parts);
+        part_slot = (int64_t)entry * a.packed.kv_heads + r;
+        first_head = part * a.packed.group / a.parts;
+        group_heads = (part + 1) * a.packed.group / a.parts - first_head;
+        entry /= (unsigned)a.parts;
+      } else {
+        entry -= shared - (unsigned)a.split;
+      }
+    }
+    const PackedBlock e = packed_block(a.packed, entry);
     if (!packed_block_in_range(a.packed, e, kOwnPerBlock)) return; // the whole block
     b = 0;
-    const int r = (int)(blockIdx.x % per_entry);
-    hd = kKeysOwn ? r * a.packed.group : packed_query_head(a.packed, r);
+    hd = kKeysOwn ? r * a.packed.group + first_head : packed_query_head(a.packed, r);
     kv_hd = kKeysOwn ? r : hd / a.packed.group;
     bh = hd;
     S = e.length;
@@ -234,7 +260,19 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
   }
   const int64_t stat_row = PACKED ? packed_row : (int64_t)bh * S;
   float own_lse = 0.f, own_delta = 0.f, own_pad = 0.f; // (the padding value, floored)
-  if constexpr (!kKeysOwn) {
+  // PACKED, own queries: the rows of O, from which delta is worked out while the first
+  // tiles are on their way (the loads are issued here)
+  constexpr bool kOwnDelta = PACKED && !kKeysOwn;
+  Frag own_o[kOwnDelta ? kSteps : 1];
+  if constexpr (kOwnDelta) {
+    const BufRsrc rs = make_rsrc(slice(a.out, a.sout, hd), slice_bytes(a.sout));
+    const uint32_t row = (uint32_t)a.sout.s * sizeof(T);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      own_o[s] = __builtin_bit_cast(Frag, __builtin_amdgcn_raw_buffer_load_b128(
+                                              rs, (uint32_t)own * row + (uint32_t)(16 * s + 8 * half) * sizeof(T), 0, 0));
+    if (own < S) own_lse = a.lse[stat_row + own];
+  } else if constexpr (!kKeysOwn) {
     if (own < S) {
       own_lse = a.lse[stat_row + own];
       own_delta = a.delta[stat_row + own];
@@ -605,6 +643,26 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
       scheduled_tile.template operator()<MASKED>();
     }
   };
+  // delta = sum_d dO O of the lane's query: eight features at a time, the halves of the wave and the
+  // steps added pair by pair (attention_delta_kernel's order, to the bit)
+  auto finish_delta = [&]() __attribute__((always_inline)) {
+    if constexpr (kOwnDelta) {
+      float part[kSteps];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x = __builtin_fmaf(static_cast<float>(own_o[s][i]), static_cast<float>(own2[s][i]), x);
+        part[s] = halves_sum(x);
+      }
+#pragma unroll
+      for (int step = 1; step < kSteps; step *= 2)
+#pragma unroll
+        for (int s = 0; s < kSteps; s += 2 * step) part[s] += part[s + step];
+      own_delta = part[0];
+      if (own < S && half == 0) a.delta_out[stat_row + own] = own_delta;
+    }
+  };
   // The walk over the tiles of one head of the other kind.
   auto walk = [&]() __attribute__((always_inline)) {
     // prologue: the first two tiles on their way
@@ -615,6 +673,7 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
       for (int it = 0; it < kItems; ++it) stage_item(it);
     }
     t = first_tile;
+    finish_delta();
 
     // the block's first tile: nothing to accumulate yet; plain order
     {
@@ -660,7 +719,7 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
   };
   if constexpr (PACKED && kKeysOwn) {
 #pragma unroll 1
-    for (int g = 0; g < a.packed.group; ++g) {
+    for (int g = 0; g < group_heads; ++g) {
       if (g > 0) __syncthreads(); // every wave has read its last operands: the buffers may be written again
       start_sources(o1_p + g * st_o1.h, o2_p + g * st_o2.h, stat_row + g * stat_step);
       walk();
@@ -674,6 +733,19 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
   typedef T Out4 __attribute__((ext_vector_type(4)));
   auto store = [&](const f32x16 (&sums)[kBlocksD], void *out_base, const Strides3 &st_out, float factor)
                    __attribute__((always_inline)) {
+    if constexpr (PACKED && kKeysOwn) {
+      if (part_slot >= 0) {
+        float *fp = a.partial + ((part_slot * 2 + (out_base == a.dv ? 1 : 0)) * kOwnPerBlock + 32 * wave + col) * (int64_t)D;
+#pragma unroll
+        for (int i = 0; i < kBlocksD; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4 *>(fp + 32 * i + 8 * j + 4 * half) =
+                make_float4(sums[i][4 * j] * factor, sums[i][4 * j + 1] * factor, sums[i][4 * j + 2] * factor,
+                            sums[i][4 * j + 3] * factor);
+        return;
+      }
+    }
     T *op = static_cast<T *>(out_base) + b * st_out.b + (kKeysOwn ? kv_hd : hd) * st_out.h + (start + own) * st_out.s;
 #pragma unroll
     for (int i = 0; i < kBlocksD; ++i)

@@ -70,7 +70,7 @@ __device__ __forceinline__ void store_e4m3(unsigned char *pages, unsigned char *
     w[j] = (uint32_t)v;
   }
   if (slot >= 0) {
-    *reinterpret_cast<u32x2 *>(pages + slot * D + 8 * part) = w;
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x2 *>(pages + slot * D + 8 * part));
     if (part == 0) scales[slot] = (unsigned char)(e + 127);
   }
 }
@@ -85,16 +85,17 @@ __global__ __launch_bounds__(kBlockThreads) void paged_kv_write_kernel(const Pag
   const int head = (int)(row - t * a.map.kv_heads);
   if (t >= a.tokens) return; // (whole groups of lanes)
   using V = RawVec<T, 8>;
-  const V k = *reinterpret_cast<const V *>(static_cast<const T *>(a.key) + t * a.key_token + head * a.key_head + 8 * part);
-  const V v =
-      *reinterpret_cast<const V *>(static_cast<const T *>(a.value) + t * a.value_token + head * a.value_head + 8 * part);
+  const V k = __builtin_nontemporal_load(
+      reinterpret_cast<const V *>(static_cast<const T *>(a.key) + t * a.key_token + head * a.key_head + 8 * part));
+  const V v = __builtin_nontemporal_load(
+      reinterpret_cast<const V *>(static_cast<const T *>(a.value) + t * a.value_token + head * a.value_head + 8 * part));
   const int64_t slot = slot_of(a, t, head);
   if constexpr (E4M3) {
     store_e4m3<T, D>(static_cast<unsigned char *>(a.key_pages), a.key_scales, slot, part, k);
     store_e4m3<T, D>(static_cast<unsigned char *>(a.value_pages), a.value_scales, slot, part, v);
   } else if (slot >= 0) {
-    *reinterpret_cast<V *>(static_cast<T *>(a.key_pages) + slot * D + 8 * part) = k;
-    *reinterpret_cast<V *>(static_cast<T *>(a.value_pages) + slot * D + 8 * part) = v;
+    __builtin_nontemporal_store(k, reinterpret_cast<V *>(static_cast<T *>(a.key_pages) + slot * D + 8 * part));
+    __builtin_nontemporal_store(v, reinterpret_cast<V *>(static_cast<T *>(a.value_pages) + slot * D + 8 * part));
   }
 }
 
@@ -118,7 +119,8 @@ __global__ __launch_bounds__(kBlockThreads) void paged_kv_read_kernel(const Page
     for (int i = 0; i < 8; ++i) x[i] = static_cast<T>(0.f); // (a token without a slot reads as zeros)
     if (slot >= 0) {
       if constexpr (E4M3) {
-        const u32x2 w = *reinterpret_cast<const u32x2 *>(static_cast<const unsigned char *>(pages) + slot * D + 8 * part);
+        const u32x2 w = __builtin_nontemporal_load(
+            reinterpret_cast<const u32x2 *>(static_cast<const unsigned char *>(pages) + slot * D + 8 * part));
         const float scale = exponent_to_scale((which ? a.value_scales : a.key_scales)[slot]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -126,14 +128,14 @@ __global__ __launch_bounds__(kBlockThreads) void paged_kv_read_kernel(const Page
           x[4 * j] = lo[0], x[4 * j + 1] = lo[1], x[4 * j + 2] = hi[0], x[4 * j + 3] = hi[1];
         }
       } else {
-        x = *reinterpret_cast<const V *>(static_cast<const T *>(pages) + slot * D + 8 * part);
+        x = __builtin_nontemporal_load(reinterpret_cast<const V *>(static_cast<const T *>(pages) + slot * D + 8 * part));
       }
     }
     out[which] = x;
   }
   const int64_t at = row * D + 8 * part; // (dense outputs)
-  *reinterpret_cast<V *>(static_cast<T *>(a.key) + at) = out[0];
-  *reinterpret_cast<V *>(static_cast<T *>(a.value) + at) = out[1];
+  __builtin_nontemporal_store(out[0], reinterpret_cast<V *>(static_cast<T *>(a.key) + at));
+  __builtin_nontemporal_store(out[1], reinterpret_cast<V *>(static_cast<T *>(a.value) + at));
 }
 
 template <typename T, int D, bool WRITE>

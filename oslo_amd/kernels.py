@@ -819,12 +819,13 @@ def attention_packed_backward(grad_out, query, key, value, out, lse, packed, sca
     dk, dv = (_packed_empty(t, hkv, d, packed, query) for _ in range(2))
     if packed.total and h:
         lib = _lib.load()
-        ws = torch.empty(lib.oslo_attention_packed_bwd_workspace_bytes(t, h) // 4, dtype=torch.float32,
-                         device=query.device)
+        split, parts = packed.shared_blocks(h, hkv, d, window)
+        ws = torch.empty(lib.oslo_attention_packed_bwd_workspace_bytes(t, h, hkv, d, split, parts) // 4,
+                         dtype=torch.float32, device=query.device)
         with _on_device(q):
             _lib.check(lib.oslo_attention_packed_bwd(
                 _ptr(dq), _ptr(dk), _ptr(dv), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(ws),
-                _ptr(packed.blocks[0]), _ptr(packed.blocks[1]), packed.blocks.shape[1], scale, t,
+                _ptr(packed.blocks[0]), _ptr(packed.blocks[1]), packed.blocks.shape[1], split, parts, scale, t,
                 packed.max_length, h, hkv, d, window, _token_strides(q, k, v, o, g, dq, dk, dv), code, _stream(q)))
     return dq, dk, dv
 

@@ -8,6 +8,7 @@ import numpy as np
 import torch
 
 PACKED_BLOCK = 128  # positions of a sequence one block of the attention kernels takes
+CUS = 256  # of an MI355X
 
 
 class PackedSequences(object):
@@ -38,11 +39,39 @@ class PackedSequences(object):
         queries = n[owner] - block * PACKED_BLOCK
         order = [np.argsort(-keys, kind="stable"), np.argsort(-queries, kind="stable")]
         self.blocks = torch.from_numpy(np.stack([entries[o] for o in order])).to(device)
+        self._queries = queries[order[1]]  # of the blocks with most queries first: how many are left
+        self._shared = {}
         self._positions = self._sequence = None
 
     @property
     def device(self):
         return self.blocks.device
+
+    def shared_blocks(self, heads, kv_heads, head_dim, window=0):
+        """(split, parts) for the gradients of keys and values: the first ``split``
+        blocks of the list are worked on by ``parts`` kernel blocks each, which take
+        the query heads of a group between them, because one alone would go on
+        when the rest of the card has finished. Host arithmetic only."""
+        key = (heads, kv_heads, head_dim, window)
+        found = self._shared.get(key)
+        if found is None:
+            found = self._shared[key] = self._share(heads // kv_heads, kv_heads, 2 if head_dim == 64 else 1, window)
+        return found
+
+    def _share(self, group, kv_heads, blocks_per_cu, window):
+        if group == 1 or not len(self._queries):
+            return 0, 1
+        # tiles of 32 queries a block walks per head, and two for its start and end
+        tiles = -(-np.minimum(self._queries, window + PACKED_BLOCK - 1 if window else self._queries) // 32) + 2
+        work = tiles * group
+        average = work.sum() * kv_heads / (CUS * blocks_per_cu)  # a CU's, if it were spread evenly
+        limit = 0.75 * average
+        # (below a tenth more than the average the last blocks hide in the others' unevenness; the sums of a
+        # shared block cost about 32 tiles of time)
+        if work[0] <= max(1.1 * average, work[0] / group + 32):
+            return 0, 1
+        parts = next(p for p in range(2, group + 1) if group % p == 0 and (work[0] / p <= max(limit, 32) or p == group))
+        return int((work > max(limit, 32)).sum()), parts
 
     def _per_token(self, values):
         return torch.from_numpy(values.astype(np.int32)).to(self.device)

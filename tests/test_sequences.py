@@ -31,6 +31,19 @@ def test_blocks_cover_every_token_once(lengths):
     assert packed.positions.dtype == torch.int32 and packed.sequence.dtype == torch.int32
 
 
+def test_shared_blocks_follow_the_work():
+    """Blocks are shared where one would outlast the rest of the card, among whole heads of the group."""
+    one = PackedSequences([740, 471, 1019, 449, 983, 1387, 4095], "cpu")
+    split, parts = one.shared_blocks(32, 8, 128)
+    assert parts == 2 and 10 <= split <= 32
+    assert one.shared_blocks(32, 32, 128) == (0, 1)                          # no group to share
+    assert one.shared_blocks(32, 8, 128, window=64) == (0, 1)                # short walks
+    assert PackedSequences([4096] * 16, "cpu").shared_blocks(32, 8, 128) == (0, 1)   # enough blocks of each size
+    split, parts = PackedSequences([2000], "cpu").shared_blocks(8, 1, 64)    # 16 blocks on 256 CUs
+    assert parts == 8 and split > 8
+    assert PackedSequences([], "cpu").shared_blocks(8, 1, 64) == (0, 1)
+
+
 def test_last_tokens():
     assert PackedSequences([3, 1, 4], "cpu").last_tokens().tolist() == [2, 3, 7]
     with pytest.raises(ValueError):
@@ -113,15 +126,17 @@ def test_entry_points_screen_their_arguments():
     assert packed(tokens=2 ** 31, longest=40) == -2
     assert packed(heads=2 ** 17, kv=1, st=good) == -2
     assert packed(n=0) == 0 and packed(tokens=0) == 0 and packed(heads=0, kv=0) == 0
-    assert lib.oslo_attention_packed_bwd_workspace_bytes(40, 4) == 640
-    assert lib.oslo_attention_packed_bwd_workspace_bytes(0, 4) == 0
+    assert lib.oslo_attention_packed_bwd_workspace_bytes(40, 4, 2, 64, 0, 1) == 640
+    assert lib.oslo_attention_packed_bwd_workspace_bytes(0, 4, 2, 64, 0, 1) == 0
+    assert lib.oslo_attention_packed_bwd_workspace_bytes(41, 3, 1, 64, 2, 3) == (124 + 2 * 3 * 2 * 128 * 64) * 4
     good16 = strides(*(list(good[:8]) + [64, 256, 64, 256, 64, 128, 64, 128]))
 
-    def packed_bwd(ws=one, keys=one, lse=one, dq=one):
-        return lib.oslo_attention_packed_bwd(dq, one, one, one, one, one, one, one, lse, ws, one, keys, 1, 0.125, 40, 40,
+    def packed_bwd(ws=one, keys=one, lse=one, dq=one, split=0, parts=1):
+        return lib.oslo_attention_packed_bwd(dq, one, one, one, one, one, one, one, lse, ws, one, keys, 1, split, parts, 0.125, 40, 40,
                                              4, 2, 64, 0, good16, 2, null)
     assert packed_bwd(ws=null) == -1 and packed_bwd(keys=null) == -1 and packed_bwd(lse=null) == -1
     assert packed_bwd(ws=odd) == -2 and packed_bwd(dq=odd) == -2
+    assert packed_bwd(split=2) == -1 and packed_bwd(split=1, parts=3) == -1 and packed_bwd(parts=0) == -1
 
     # paged cache: 3 sequences of 5 pages, a pool of 20, 2 heads, pages of 16, 64 features
     st4 = strides(64, 128, 64, 128)
