@@ -594,13 +594,15 @@ int oslo_attention_prefill_bwd_stored(void *dq, void *dk, void *dv,
  * Entries that do not describe tokens of the row or exceed max_length are passed
  * over. Tokens of no sequence are neither read nor written.
  * lse: NULL, or fp32 [heads, tokens], 16-byte aligned: log2 of the row's sum of
- * 2^(log2(e) * scale * q.k), which the backward takes. Rounding as in
+ * 2^(log2(e) * scale * q.k), which the backward takes. out_low: NULL, or a
+ * tensor like out (same strides) that gets what rounding the output left out, for
+ * the backward. Rounding as in
  * oslo_attention_prefill_fwd. scale > 0. No workspace.
  * No counterpart in the reference, whose attention takes padded batches
  * (oslo/models/gptj/modeling_gptj.py:936-951).
  */
-int oslo_attention_packed_fwd(void *out, float *lse, const void *q,
-                              const void *k, const void *v,
+int oslo_attention_packed_fwd(void *out, void *out_low, float *lse,
+                              const void *q, const void *k, const void *v,
                               const int32_t *blocks, int64_t num_blocks,
                               float scale, int64_t tokens, int64_t max_length,
                               int64_t heads, int64_t kv_heads,
@@ -615,8 +617,8 @@ size_t oslo_attention_packed_bwd_workspace_bytes(int64_t tokens, int64_t heads,
                                                  int64_t split, int64_t parts);
 
 /*
- * Gradients of the packed attention from dout, the inputs, the forward's out and
- * lse: the formulas of oslo_attention_prefill_bwd per sequence; dk and dv are
+ * Gradients of the packed attention from dout, the inputs, the forward's out,
+ * out_low (or NULL: less exact where few keys carry a row) and lse: the formulas of oslo_attention_prefill_bwd per sequence; dk and dv are
  * summed over the query heads of a group in fp32, in a fixed order, and rounded
  * once. query_blocks and key_blocks hold the same entries as the forward's
  * `blocks` (most keys first, and most queries left first, run fastest).
@@ -630,10 +632,12 @@ size_t oslo_attention_packed_bwd_workspace_bytes(int64_t tokens, int64_t heads,
  */
 int oslo_attention_packed_bwd(void *dq, void *dk, void *dv, const void *dout,
                               const void *q, const void *k, const void *v,
-                              const void *out, const float *lse,
-                              float *workspace, const int32_t *query_blocks,
+                              const void *out, const void *out_low,
+                              const float *lse, float *workspace,
+                              const int32_t *query_blocks,
                               const int32_t *key_blocks, int64_t num_blocks,
-                              int64_t split, int64_t parts, float scale, int64_t tokens, int64_t max_length,
+                              int64_t split, int64_t parts, float scale,
+                              int64_t tokens, int64_t max_length,
                               int64_t heads, int64_t kv_heads,
                               int64_t head_dim, int64_t window,
                               const int64_t *strides, int dtype,

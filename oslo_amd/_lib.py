@@ -79,10 +79,10 @@ PROTOTYPES = {
         _c.c_int, [_P] * 11 + [_c.c_size_t, _P, _c.c_float, _c.c_float, _U64, _U64, _I64, _I64, _I64, _I64, _I64,
                                _c.POINTER(_c.c_int64), _c.c_int, _P]),
     "oslo_attention_packed_fwd": (
-        _c.c_int, [_P] * 6 + [_I64, _c.c_float] + [_I64] * 6 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
+        _c.c_int, [_P] * 7 + [_I64, _c.c_float] + [_I64] * 6 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
     "oslo_attention_packed_bwd_workspace_bytes": (_c.c_size_t, [_I64] * 6),
     "oslo_attention_packed_bwd": (
-        _c.c_int, [_P] * 12 + [_I64] * 3 + [_c.c_float] + [_I64] * 6 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
+        _c.c_int, [_P] * 13 + [_I64] * 3 + [_c.c_float] + [_I64] * 6 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
     "oslo_paged_kv_write": (
         _c.c_int, [_P] * 9 + [_I64] * 7 + [_c.POINTER(_c.c_int64), _c.c_int, _P]),
     "oslo_paged_kv_read": (_c.c_int, [_P] * 9 + [_I64] * 7 + [_c.c_int, _P]),

@@ -42,7 +42,7 @@ int launch_packed_dim(const PrefillArgs &a, int64_t num_blocks, int64_t head_dim
 } // namespace
 } // namespace oslo
 
-extern "C" int oslo_attention_packed_fwd(void *out, float *lse, const void *q, const void *k,
+extern "C" int oslo_attention_packed_fwd(void *out, void *out_low, float *lse, const void *q, const void *k,
                                          const void *v, const int32_t *blocks,
                                          int64_t num_blocks, float scale, int64_t tokens,
                                          int64_t max_length, int64_t heads,
@@ -56,7 +56,9 @@ extern "C" int oslo_attention_packed_fwd(void *out, float *lse, const void *q, c
   if (s != OSLO_OK) return s;
   if (num_blocks == 0 || heads == 0 || tokens == 0) return OSLO_OK;
   PrefillArgs a{};
-  a.out = out, a.q = q, a.k = k, a.v = v, a.lse = lse;
+  if (!aligned16(out_low) || !aligned16(lse))
+    return fail(OSLO_E_UNSUPPORTED, "oslo_attention_packed_fwd: lse and out_low must be 16-byte aligned");
+  a.out = out, a.out_low = out_low, a.q = q, a.k = k, a.v = v, a.lse = lse;
   a.q_h = strides[0], a.q_s = strides[1];
   a.k_h = strides[2], a.k_s = strides[3];
   a.v_h = strides[4], a.v_s = strides[5];

@@ -112,6 +112,7 @@ extern "C" size_t oslo_attention_packed_bwd_workspace_bytes(int64_t tokens, int6
 
 extern "C" int oslo_attention_packed_bwd(void *dq, void *dk, void *dv, const void *dout, const void *q,
                                          const void *k, const void *v, const void *out,
+                                         const void *out_low,
                                          const float *lse, float *workspace,
                                          const int32_t *query_blocks,
                                          const int32_t *key_blocks, int64_t num_blocks,
@@ -130,13 +131,13 @@ extern "C" int oslo_attention_packed_bwd(void *dq, void *dk, void *dv, const voi
     return fail(OSLO_E_BAD_ARG, "%s: %lld entries shared by %lld blocks each", name, (long long)split, (long long)parts);
   if (num_blocks == 0 || heads == 0 || tokens == 0) return OSLO_OK;
   if (!key_blocks || !lse || !workspace) return fail(OSLO_E_BAD_ARG, "%s: null pointer", name);
-  if (!aligned16(lse) || !aligned16(workspace))
-    return fail(OSLO_E_UNSUPPORTED, "%s: lse and the workspace must be 16-byte aligned", name);
+  if (!aligned16(lse) || !aligned16(workspace) || !aligned16(out_low))
+    return fail(OSLO_E_UNSUPPORTED, "%s: out_low, lse and the workspace must be 16-byte aligned", name);
   if (heads * tokens > (int64_t)0x7fffffff || (num_blocks + split * parts) > (int64_t)0x7fffffff / (heads * 64))
     return fail(OSLO_E_UNSUPPORTED, "%s: too many rows for one launch", name);
   auto st = [&](int i) { return Strides3{0, strides[2 * i], strides[2 * i + 1]}; };
   BwdArgs a{};
-  a.q = q, a.k = k, a.v = v, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.out = out;
+  a.q = q, a.k = k, a.v = v, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv, a.out = out, a.out_low = out_low;
   a.lse = lse, a.delta = a.delta_out = workspace;
   a.partial = workspace + (heads * tokens + 3) / 4 * 4;
   a.split = (int)split, a.parts = (int)parts;

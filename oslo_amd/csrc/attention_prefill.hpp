@@ -73,6 +73,7 @@ struct PrefillArgs {
   int query_blocks;
   int window; // 0: every key up to the query; else the last `window` of them
   DropArgs drop; // attention dropout (the DROP variants of the kernel)
+  void *out_low;     // PACKED: null, or what rounding the output left out, rounded itself; the output's strides
   PackedArgs packed; // the sequences of the PACKED variant (its batch strides, batch_heads, head_groups and query_blocks are not read)
 };
 
@@ -651,14 +652,39 @@ __global__ __launch_bounds__(kBlockThreads, D == 256 ? 1 : D == 128 ? 2 : 3) voi
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  T *const out_head = static_cast<T *>(a.out) + b * a.o_b + hd * a.o_h + o_start;
   constexpr int kRowsPerStore = kWave / kChunks;
+  auto store_rows = [&](void *to) __attribute__((always_inline)) {
+    T *const out_head = static_cast<T *>(to) + b * a.o_b + hd * a.o_h + o_start;
 #pragma unroll
-  for (int k = 0; k < 32 / kRowsPerStore; ++k) {
-    const int row = kRowsPerStore * k + lane / kChunks, piece = lane % kChunks;
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(stage + row * kOutRow + piece * 16);
-    if (wave_q0 + row < S)
-      *reinterpret_cast<u32x4 *>(out_head + (int64_t)(wave_q0 + row) * a.o_s + 8 * piece) = w;
+    for (int k = 0; k < 32 / kRowsPerStore; ++k) {
+      const int row = kRowsPerStore * k + lane / kChunks, piece = lane % kChunks;
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(stage + row * kOutRow + piece * 16);
+      if (wave_q0 + row < S)
+        *reinterpret_cast<u32x4 *>(out_head + (int64_t)(wave_q0 + row) * a.o_s + 8 * piece) = w;
+    }
+  };
+  store_rows(a.out);
+  if constexpr (PACKED) {
+    if (a.out_low != nullptr) { // (uniform)
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); // (the rows have been read)
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < kBlocksD; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          Out4 w;
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) {
+            const float x = o[i][4 * j + tt] * inv;
+            w[tt] = static_cast<T>(x - static_cast<float>(static_cast<T>(x)));
+          }
+          *reinterpret_cast<Out4 *>(stage + col * kOutRow + (32 * i + 8 * j + 4 * half) * (int)sizeof(T)) = w;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      store_rows(a.out_low);
+    }
   }
 }
 

@@ -102,7 +102,7 @@ struct BwdArgs {
   // query heads is shared by `parts` blocks (the first `split` of the list: those with most queries),
   // which leave fp32 sums [entry * parts + part][kv head][dK, dV][128][D] in `partial`.
   PackedArgs packed;
-  const void *out;
+  const void *out, *out_low; // (out_low: null, or what rounding left out of it)
   Strides3 sout;
   float *delta_out;
   float *partial;
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
   // PACKED, own queries: the rows of O, from which delta is worked out while the first
   // tiles are on their way (the loads are issued here)
   constexpr bool kOwnDelta = PACKED && !kKeysOwn;
-  Frag own_o[kOwnDelta ? kSteps : 1];
+  Frag own_o[kOwnDelta ? kSteps : 1], own_low[kOwnDelta ? kSteps : 1];
   if constexpr (kOwnDelta) {
     const BufRsrc rs = make_rsrc(slice(a.out, a.sout, hd), slice_bytes(a.sout));
     const uint32_t row = (uint32_t)a.sout.s * sizeof(T);
@@ -271,6 +271,11 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
     for (int s = 0; s < kSteps; ++s)
       own_o[s] = __builtin_bit_cast(Frag, __builtin_amdgcn_raw_buffer_load_b128(
                                               rs, (uint32_t)own * row + (uint32_t)(16 * s + 8 * half) * sizeof(T), 0, 0));
+    const BufRsrc low = make_rsrc(slice(a.out_low, a.sout, hd), a.out_low != nullptr ? slice_bytes(a.sout) : 0u); // (null: zeros)
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      own_low[s] = __builtin_bit_cast(Frag, __builtin_amdgcn_raw_buffer_load_b128(
+                                                low, (uint32_t)own * row + (uint32_t)(16 * s + 8 * half) * sizeof(T), 0, 0));
     if (own < S) own_lse = a.lse[stat_row + own];
   } else if constexpr (!kKeysOwn) {
     if (own < S) {
@@ -643,8 +648,11 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
       scheduled_tile.template operator()<MASKED>();
     }
   };
-  // delta = sum_d dO O of the lane's query: eight features at a time, the halves of the wave and the
-  // steps added pair by pair (attention_delta_kernel's order, to the bit)
+  // delta = sum_d dO O of the lane's query, eight features at a time, then the halves of the wave and the
+  // steps pair by pair. O is taken with what its rounding left out: delta stands against dP in
+  // every dS of the row, and where the probabilities are concentrated (a window of a few keys, the first
+  // tokens of a sequence) the rounding of O alone doubled the error of dQ and dK (bf16, a window of 2:
+  // 0.0039 of their norm instead of 0.0025).
   auto finish_delta = [&]() __attribute__((always_inline)) {
     if constexpr (kOwnDelta) {
       float part[kSteps];
@@ -652,7 +660,8 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
       for (int s = 0; s < kSteps; ++s) {
         float x = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x = __builtin_fmaf(static_cast<float>(own_o[s][i]), static_cast<float>(own2[s][i]), x);
+        for (int i = 0; i < 8; ++i)
+          x = __builtin_fmaf(static_cast<float>(own_o[s][i]) + static_cast<float>(own_low[s][i]), static_cast<float>(own2[s][i]), x);
         part[s] = halves_sum(x);
       }
 #pragma unroll

@@ -684,23 +684,24 @@ class FusedPrefillAttention(object):
 
 class _PackedAttention(torch.autograd.Function):
     """The packed attention with its backward, which recomputes the
-    probabilities from the log-sum-exp of every row. It cannot be differentiated
+    probabilities from the log-sum-exp of every row (and keeps what rounding
+    left out of the output, 16 bits a feature, for the row sums it needs). It cannot be differentiated
     again, and it always computes all three gradients."""
 
     @staticmethod
     def forward(ctx, query, key, value, packed, scale, window):
-        out, lse = get_custom_kernels().attention_packed_forward(query, key, value, packed, scale, window,
-                                                                 want_lse=True)
-        ctx.save_for_backward(query, key, value, out, lse)
+        out, low, lse = get_custom_kernels().attention_packed_forward(query, key, value, packed, scale, window,
+                                                                      want_lse=True)
+        ctx.save_for_backward(query, key, value, out, low, lse)
         ctx.args = (packed, float(scale), int(window))
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        query, key, value, out, lse = ctx.saved_tensors
+        query, key, value, out, low, lse = ctx.saved_tensors
         packed, scale, window = ctx.args
-        dq, dk, dv = get_custom_kernels().attention_packed_backward(grad_out, query, key, value, out, lse, packed,
+        dq, dk, dv = get_custom_kernels().attention_packed_backward(grad_out, query, key, value, out, low, lse, packed,
                                                                     scale, window)
         return dq, dk, dv, None, None, None
 

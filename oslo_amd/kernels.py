@@ -785,27 +785,29 @@ def attention_packed_forward(query, key, value, packed, scale, window=0, want_ls
     """Causal attention over the sequences ``packed`` (a ``PackedSequences``)
     laid one behind the other: query [T, H, D], key and value [T, Hkv, D]
     fp16/bf16 views (features contiguous), H a multiple of Hkv. Returns
-    [T, H, D] (rows behind the last sequence: zeros), with ``want_lse`` also the
-    fp32 [H, T] log2-sum-exp that ``attention_packed_backward`` takes."""
+    [T, H, D] (rows behind the last sequence: zeros), with ``want_lse`` also what
+    ``attention_packed_backward`` takes: the part of the output that its
+    rounding left out, [T, H, D], and the fp32 [H, T] log2-sum-exp."""
     code = _packed_args(query, key, value, packed)
     t, h, d = query.shape
     q, k, v = _packed_strided(query), _packed_strided(key), _packed_strided(value)
     out = _packed_empty(t, h, d, packed, query)
+    low = torch.empty((t, h, d), dtype=query.dtype, device=query.device) if want_lse else None
     lse = torch.empty((h, t), dtype=torch.float32, device=query.device) if want_lse else None
     if packed.total and h:
         blocks = packed.blocks
         with _on_device(q):
             _lib.check(_lib.load().oslo_attention_packed_fwd(
-                out.data_ptr(), _ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), blocks.shape[1],
-                scale, t, packed.max_length, h, k.shape[1], d, window, _token_strides(q, k, v, out), code, _stream(q)))
-    return (out, lse) if want_lse else out
+                out.data_ptr(), _ptr(low), _ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(),
+                blocks.shape[1], scale, t, packed.max_length, h, k.shape[1], d, window, _token_strides(q, k, v, out), code, _stream(q)))
+    return (out, low, lse) if want_lse else out
 
 
-def attention_packed_backward(grad_out, query, key, value, out, lse, packed, scale, window=0):
+def attention_packed_backward(grad_out, query, key, value, out, out_low, lse, packed, scale, window=0):
     """Gradients of ``attention_packed_forward`` with respect to query, key and
     value (dense; rows behind the last sequence: zeros)."""
     code = _packed_args(query, key, value, packed)
-    for what, x in (("grad_out", grad_out), ("out", out)):
+    for what, x in (("grad_out", grad_out), ("out", out), ("out_low", out_low)):
         _device_tensor(x, what, query)
         if x.shape != query.shape or x.dtype != query.dtype:
             raise RuntimeError(f"{what} must be like query")
@@ -814,6 +816,7 @@ def attention_packed_backward(grad_out, query, key, value, out, lse, packed, sca
     hkv = key.shape[1]
     _require(lse.dtype == torch.float32 and tuple(lse.shape) == (h, t) and lse.is_contiguous(),
              "lse must be the fp32 [H, T] tensor of the forward")
+    _require(out.is_contiguous() and out_low.is_contiguous(), "out and out_low must be the forward's")
     q, k, v, o, g = (_packed_strided(x) for x in (query, key, value, out, grad_out))
     dq = _packed_empty(t, h, d, packed, query)
     dk, dv = (_packed_empty(t, hkv, d, packed, query) for _ in range(2))
@@ -824,8 +827,8 @@ def attention_packed_backward(grad_out, query, key, value, out, lse, packed, sca
                          dtype=torch.float32, device=query.device)
         with _on_device(q):
             _lib.check(lib.oslo_attention_packed_bwd(
-                _ptr(dq), _ptr(dk), _ptr(dv), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(ws),
-                _ptr(packed.blocks[0]), _ptr(packed.blocks[1]), packed.blocks.shape[1], split, parts, scale, t,
+                _ptr(dq), _ptr(dk), _ptr(dv), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(o),
+                _ptr(out_low), _ptr(lse), _ptr(ws), _ptr(packed.blocks[0]), _ptr(packed.blocks[1]), packed.blocks.shape[1], split, parts, scale, t,
                 packed.max_length, h, hkv, d, window, _token_strides(q, k, v, o, g, dq, dk, dv), code, _stream(q)))
     return dq, dk, dv
 

@@ -110,7 +110,7 @@ def test_entry_points_screen_their_arguments():
 
     def packed(blocks=one, n=1, scale=0.125, tokens=40, longest=40, heads=4, kv=2, d=64, window=0, st=good, dtype=2,
                out=one, q=one):
-        return lib.oslo_attention_packed_fwd(out, null, q, one, one, blocks, n, scale, tokens, longest, heads, kv, d,
+        return lib.oslo_attention_packed_fwd(out, null, null, q, one, one, blocks, n, scale, tokens, longest, heads, kv, d,
                                              window, st, dtype, null)
     assert packed(n=-1) == -1 and packed(tokens=-1) == -1 and packed(window=-1) == -1
     assert packed(dtype=0) == -2 and packed(dtype=7) == -1
@@ -132,7 +132,7 @@ def test_entry_points_screen_their_arguments():
     good16 = strides(*(list(good[:8]) + [64, 256, 64, 256, 64, 128, 64, 128]))
 
     def packed_bwd(ws=one, keys=one, lse=one, dq=one, split=0, parts=1):
-        return lib.oslo_attention_packed_bwd(dq, one, one, one, one, one, one, one, lse, ws, one, keys, 1, split, parts, 0.125, 40, 40,
+        return lib.oslo_attention_packed_bwd(dq, one, one, one, one, one, one, one, null, lse, ws, one, keys, 1, split, parts, 0.125, 40, 40,
                                              4, 2, 64, 0, good16, 2, null)
     assert packed_bwd(ws=null) == -1 and packed_bwd(keys=null) == -1 and packed_bwd(lse=null) == -1
     assert packed_bwd(ws=odd) == -2 and packed_bwd(dq=odd) == -2
