@@ -34,6 +34,6 @@ from .modeling_gpt2 import GPT2Config, GPT2LMHeadModel  # noqa: F401
 from .modeling_gpt_neo import GPTNeoConfig, GPTNeoForCausalLM  # noqa: F401
 from .modeling_gptj import GPTJConfig, GPTJForCausalLM  # noqa: F401
 from .modeling_utils import DecodeState, StaticKV  # noqa: F401
-from .sequences import PackedSequences, PagedKV  # noqa: F401
+from .sequences import PackedSequences, PagedKV, PagedState  # noqa: F401
 
 __version__ = "0.1.0"

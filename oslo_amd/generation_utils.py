@@ -1,17 +1,24 @@
-"""``model.generate``: greedy and beam-search decoding over a key/value cache,
+"""``model.generate``: greedy, sampled and beam-search decoding over a key/value cache,
 with the repeated n-gram ban either on the host (the HuggingFace processor) or
 on the device (``FusedNoRepeatNGramLogitsProcessor``).
 
 The reference's generation code is a fork of HuggingFace's GenerationMixin
 (oslo/generation_utils.py) whose one addition on this path is the switch
 ``fused_no_repeat_ngram_blocking`` (:423-434, :753-757). This file is not that
-fork: it restates the two decoding modes the reference's kernel-fusion test
+fork: it restates the decoding modes the reference's kernel-fusion test
 uses (tests/gpt2/gpt2_test_kernel_fusion.py:26-33: ``max_length``,
 ``min_length``, ``num_beams``, ``no_repeat_ngram_size``) with the same
 argument names and the same beam-search rule (oslo/generation_utils.py:
 1913-1990 and HuggingFace's BeamSearchScorer), for prompts of equal length
-without padding. Sampling, beam groups, constraints and the other logits
+without padding; and, with ``do_sample``, drawing from the distribution that
+temperature, top-k, top-p and min-p leave (one launch per step, where the
+reference chains its warpers and torch.multinomial,
+oslo/generation_utils.py). Beam groups, constraints and the other logits
 processors are not provided.
+
+A list of prompts of different lengths is taken too (no counterpart in the
+reference, which pads): the prompts run through the model packed into one row,
+and their steps over a paged key/value cache, in 16 or 8 bits.
 
 While no sequence can end (no ``eos_token_id``, or the length is still below
 ``min_length``) a step does not synchronise with the host: the beam
@@ -29,7 +36,8 @@ steps without a graph (on any device).
 
 import torch
 
-from .fused_kernels_utils import FusedNoRepeatNGramLogitsProcessor
+from .fused_kernels_utils import FusedLinearRows, FusedNoRepeatNGramLogitsProcessor, FusedSampling
+from .sequences import PackedSequences, PagedState
 
 
 class DynamicDecoder(object):
@@ -150,6 +158,65 @@ class StaticDecoder(object):
         return logits
 
 
+class PagedDecoder(object):
+    """Steps of sequences of different lengths over paged caches; optionally each
+    step is one graph replay."""
+
+    def __init__(self, model, prompts, capacity, graph, quantized):
+        config, weight = model.config, model.transformer.wte.weight
+        heads = config.num_attention_heads
+        self.model, self.graph, self.captured = model, graph, None
+        lengths = [p.numel() for p in prompts]
+        self.packed = PackedSequences(lengths, weight.device)
+        self.state = PagedState(lengths, capacity, len(model.transformer.h), heads, config.hidden_size // heads,
+                                weight.dtype, weight.device, quantized=quantized)
+        self.row = torch.cat(list(prompts))[None]
+        self.token = torch.zeros((1, len(lengths)), dtype=self.row.dtype, device=weight.device)
+
+    def prompt(self):
+        """All prompts in one forward -> the logits behind each, [sequences, vocabulary]."""
+        model = self.model
+        h = model.transformer(self.row, None, self.state.prompt_layers(self.packed))[0]
+        h = h[0].index_select(0, self.packed.last_tokens())  # (only these rows go through the head)
+        if getattr(model, "fused_lm_head", False) and not model.training:
+            return FusedLinearRows.project(model.lm_head, h)
+        return model.lm_head(h)
+
+    def _run(self):
+        logits = self.model(self.token, past_key_values=self.state.begin_step())["logits"][0]
+        self.state.end_step()
+        return logits
+
+    def _capture(self):
+        state, device = self.state, self.token.device
+        lengths = state.lengths.clone()
+        # warm-up on a side stream: lazy initialisation must not happen inside the
+        # capture. It writes the slots that the step itself writes again.
+        side = torch.cuda.Stream(device=device)
+        side.wait_stream(torch.cuda.current_stream(device))
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                self._run()
+                state.lengths.copy_(lengths)
+        torch.cuda.current_stream(device).wait_stream(side)
+        torch.cuda.synchronize(device)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = self._run()
+        return graph, logits
+
+    def step(self, tokens):
+        """The next token of every sequence, [sequences] -> the logits behind them."""
+        self.token.copy_(tokens[None])
+        if not self.graph:
+            return self._run()
+        if self.captured is None:
+            self.captured = self._capture()
+        graph, logits = self.captured
+        graph.replay()
+        return logits
+
+
 class _HostNoRepeatNGram(object):
     """The unfused ban: HuggingFace's NoRepeatNGramLogitsProcessor, which walks
     the token lists on the host (what the reference uses when the switch is
@@ -197,7 +264,34 @@ class GenerationMixin(object):
     @torch.no_grad()
     def generate(self, input_ids, max_length=20, min_length=0, num_beams=1, no_repeat_ngram_size=None,
                  fused_no_repeat_ngram_blocking=None, eos_token_id=None, pad_token_id=None,
-                 length_penalty=1.0, use_cache=True, static_cache=None, graph=False):
+                 length_penalty=1.0, use_cache=True, static_cache=None, graph=False, do_sample=False,
+                 temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, quantized_cache=False):
+        """``input_ids`` [batch, length] -> [batch, up to max_length]. ``do_sample``
+        draws the tokens as ``FusedSampling`` does (its ``temperature``, ``top_k``,
+        ``top_p``, ``min_p``), by uniform numbers from ``generator``.
+
+        With a list of prompts (1-D tensors of any lengths below ``max_length``;
+        fused models) the sequences come back as a list, each cut behind its
+        ``eos_token_id``. Their cache is paged; ``quantized_cache`` keeps it in 8 bits."""
+        if do_sample and num_beams != 1:
+            raise ValueError("generate: do_sample goes with num_beams=1")
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+        def choose(scores):
+            if not do_sample:
+                return scores.argmax(dim=-1)
+            uniforms = torch.rand(scores.size(0), generator=generator, device=scores.device)
+            # (a row without any finite score has no token, -1: 0, which argmax gives there)
+            return FusedSampling.apply(scores, uniforms, **settings)[0].clamp_(min=0)
+
+        if isinstance(input_ids, (list, tuple)):
+            if num_beams != 1 or no_repeat_ngram_size or static_cache or not use_cache:
+                raise ValueError("generate: a list of prompts is decoded over its own paged cache, without beams and "
+                                 "n-gram blocking")
+            return self._generate_sequences(input_ids, max_length, min_length, eos_token_id, choose, graph,
+                                            quantized_cache)
+        if quantized_cache:
+            raise ValueError("generate: quantized_cache goes with a list of prompts")
         if input_ids.dim() != 2:
             raise ValueError("generate: input_ids must be [batch, length]")
         if input_ids.size(1) >= max_length:
@@ -240,7 +334,7 @@ class GenerationMixin(object):
             return s
 
         if num_beams == 1:
-            return self._greedy_search(input_ids, max_length, scores_of, eos_token_id, pad_token_id, decoder)
+            return self._search(input_ids, max_length, scores_of, choose, eos_token_id, pad_token_id, decoder)
         return self._beam_search(input_ids, max_length, min_length, num_beams, scores_of, eos_token_id,
                                  pad_token_id, length_penalty, decoder)
 
@@ -265,10 +359,10 @@ class GenerationMixin(object):
         self.__dict__.pop("_kept_decoder", None)
 
     @staticmethod
-    def _greedy_search(ids, max_length, scores_of, eos_token_id, pad_token_id, decoder):
+    def _search(ids, max_length, scores_of, choose, eos_token_id, pad_token_id, decoder):
         unfinished = None if eos_token_id is None else torch.ones(ids.size(0), dtype=torch.bool, device=ids.device)
         while ids.size(1) < max_length:
-            nxt = scores_of(ids, decoder.step(ids)).argmax(dim=-1)
+            nxt = choose(scores_of(ids, decoder.step(ids)))
             if unfinished is not None:
                 nxt = torch.where(unfinished, nxt, torch.full_like(nxt, pad_token_id))
                 unfinished = unfinished & (nxt != eos_token_id)
@@ -276,6 +370,47 @@ class GenerationMixin(object):
             if unfinished is not None and not bool(unfinished.any()):
                 break
         return ids
+
+    def _generate_sequences(self, prompts, max_length, min_length, eos_token_id, choose, graph, quantized):
+        if not prompts:
+            return []
+        if any(p.dim() != 1 or not 0 < p.numel() < max_length for p in prompts):
+            raise ValueError("generate: a list of prompts holds 1-D tensors of 1 to "
+                             f"max_length - 1 = {max_length - 1} tokens")
+        if not all(p.is_cuda for p in prompts):
+            raise RuntimeError("generate: a list of prompts needs the model and the prompts on a ROCm device")
+        if graph and self.training:
+            raise RuntimeError("generate: graph=True captures inference: call model.eval() first")
+        decoder = PagedDecoder(self, prompts, max_length, graph, quantized)
+        lengths = [p.numel() for p in prompts]
+        dev = prompts[0].device
+        steps = max_length - min(lengths)
+        if eos_token_id is not None:
+            left = torch.tensor([max_length - n for n in lengths], device=dev)  # tokens until a sequence is full
+            early = torch.tensor([min_length - n for n in lengths], device=dev)  # tokens before it may end
+            running = torch.ones(len(lengths), dtype=torch.bool, device=dev)
+        logits, new = decoder.prompt(), []
+        for step in range(steps):
+            if eos_token_id is not None and step < min_length - min(lengths):
+                logits = logits.clone()
+                logits[:, eos_token_id].masked_fill_(early > step, float("-inf"))
+            nxt = choose(logits)
+            new.append(nxt)
+            if eos_token_id is not None:
+                running = running & (nxt != eos_token_id) & (left > step + 1)
+                if not bool(running.any()):
+                    break
+            if step + 1 < steps:
+                logits = decoder.step(nxt)
+        new = torch.stack(new, dim=1)
+        out = []
+        for row, prompt in enumerate(prompts):
+            tokens = new[row, :max_length - lengths[row]]
+            if eos_token_id is not None:
+                ends = (tokens == eos_token_id).nonzero()
+                tokens = tokens[:int(ends[0]) + 1] if ends.numel() else tokens
+            out.append(torch.cat([prompt, tokens.to(prompt.dtype)]))
+        return out
 
     def _beam_search(self, input_ids, max_length, min_length, num_beams, scores_of, eos_token_id, pad_token_id,
                      length_penalty, decoder):

@@ -799,7 +799,8 @@ def attention_packed_forward(query, key, value, packed, scale, window=0, want_ls
         with _on_device(q):
             _lib.check(_lib.load().oslo_attention_packed_fwd(
                 out.data_ptr(), _ptr(low), _ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(),
-                blocks.shape[1], scale, t, packed.max_length, h, k.shape[1], d, window, _token_strides(q, k, v, out), code, _stream(q)))
+                blocks.shape[1], scale, t, packed.max_length, h, k.shape[1], d, window, _token_strides(q, k, v, out),
+                code, _stream(q)))
     return (out, low, lse) if want_lse else out
 
 
@@ -828,7 +829,8 @@ def attention_packed_backward(grad_out, query, key, value, out, out_low, lse, pa
         with _on_device(q):
             _lib.check(lib.oslo_attention_packed_bwd(
                 _ptr(dq), _ptr(dk), _ptr(dv), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(o),
-                _ptr(out_low), _ptr(lse), _ptr(ws), _ptr(packed.blocks[0]), _ptr(packed.blocks[1]), packed.blocks.shape[1], split, parts, scale, t,
+                _ptr(out_low), _ptr(lse), _ptr(ws), _ptr(packed.blocks[0]), _ptr(packed.blocks[1]),
+                packed.blocks.shape[1], split, parts, scale, t,
                 packed.max_length, h, hkv, d, window, _token_strides(q, k, v, o, g, dq, dk, dv), code, _stream(q)))
     return dq, dk, dv
 

@@ -18,8 +18,9 @@ from .fused_kernels_utils import (FusedBiasActivation, FusedBiasDropout, FusedBi
                                  FusedMergeHeads,
                                  FusedScaleMaskSoftmax,
                                  FusedScaleMaskSoftmaxDropout, FusedSplitHeads)
-from .modeling_utils import (ACT2FN, Conv1D, LayerPolicy, PreTrainedModel, StaticKV, additive_attention_mask,
-                             append_kv, causal_lm_loss, static_cache_mask)
+from .modeling_utils import (ACT2FN, Conv1D, LayerPolicy, PreTrainedModel, SequenceLayer, StaticKV,
+                             additive_attention_mask, append_kv, causal_lm_loss, packed_past, sequence_attention,
+                             sequence_positions, static_cache_mask)
 
 
 @dataclass
@@ -173,6 +174,14 @@ class FusedGPT2Attention(GPT2Attention):
                 output_attentions=False, residual=None):
         """``residual``: added to the output (the residual connection of the
         block, which a decoding step takes into the projection's launch)."""
+        if isinstance(layer_past, SequenceLayer):
+            if encoder_hidden_states is not None or self.is_cross_attention:
+                raise RuntimeError("packed and paged attention are self-attention")
+            qkv = FusedLinearRows.project_conv1d(self.c_attn, hidden_states)
+            query, key, value = qkv.view(qkv.shape[1], 3, self.num_heads, self.head_dim).unbind(1)
+            out = sequence_attention(self, layer_past, query, key, value, self._attention_scale(value), None, head_mask,
+                                     attention_mask, output_attentions)
+            return self._output(out, residual), layer_past
         query, key, value, present = self._project_qkv(hidden_states, layer_past, encoder_hidden_states, use_cache)
         if encoder_hidden_states is not None:
             attention_mask = encoder_attention_mask
@@ -213,6 +222,11 @@ class FusedGPT2Attention(GPT2Attention):
             out = FusedMergeHeads.apply(out)
         else:
             out = self._merge_heads(out, self.num_heads, self.head_dim)
+        out = self._output(out, residual)
+        return (out, present, w) if output_attentions else (out, present)
+
+    def _output(self, out, residual):
+        """The output projection with its bias, dropout and the block's residual addition."""
         if FusedLinearRows.is_available(out, self.c_proj.weight, self.c_proj.bias, conv1d=True) and not (
                 self.training and self.resid_dropout.p > 0.0):
             out = FusedLinearRows.apply(out, self.c_proj.weight, self.c_proj.bias, conv1d=True,
@@ -224,7 +238,7 @@ class FusedGPT2Attention(GPT2Attention):
             else:  # with the block's residual addition in the same pass
                 out = FusedBiasDropoutResidual.apply(out, self.c_proj.bias, residual, self.training,
                                                      self.resid_dropout.p)
-        return (out, present, w) if output_attentions else (out, present)
+        return out
 
 
 class GPT2MLP(nn.Module):
@@ -293,6 +307,8 @@ class FusedGPT2Block(GPT2Block):
     (oslo/models/gpt2/configuration_gpt2.py:272-284); the arithmetic is that
     of oslo/models/gpt2/modeling_gpt2.py:420-481."""
 
+    takes_sequences = True
+
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         if not (isinstance(self.attn, FusedGPT2Attention) and isinstance(self.mlp, FusedGPT2MLP)):
             return super().forward(hidden_states, layer_past, attention_mask, head_mask, use_cache)
@@ -320,7 +336,10 @@ class GPT2Model(nn.Module):
         self.ln_f = nn.LayerNorm(config.hidden_size, eps=config.layer_norm_epsilon)
 
     def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False):
-        if past_key_values is not None and isinstance(past_key_values[0], StaticKV):
+        pos = sequence_positions(past_key_values, input_ids, self.wpe.num_embeddings, self.h)
+        if pos is not None:
+            pass  # sequences of different lengths
+        elif past_key_values is not None and isinstance(past_key_values[0], StaticKV):
             pos = past_key_values[0].state.pos
         else:
             past_len = 0 if past_key_values is None else past_key_values[0][0].size(-2)
@@ -348,9 +367,13 @@ class GPT2LMHeadModel(PreTrainedModel):
     def get_layer_policies(self):
         return [GPT2LayerPolicy]
 
-    def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False, labels=None):
+    def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False, labels=None, packed=None):
+        """``packed``: a ``PackedSequences``: input_ids [1, tokens] are its sequences
+        one behind the other, none of which sees another (fused modules only)."""
+        if packed is not None:
+            past_key_values = packed_past(len(self.transformer.h), packed, past_key_values, attention_mask, use_cache)
         h, presents = self.transformer(input_ids, attention_mask, past_key_values, use_cache)
         fused_head = getattr(self, "fused_lm_head", False) and not self.training
         logits = FusedLinearRows.project(self.lm_head, h) if fused_head else self.lm_head(h)
-        loss = causal_lm_loss(logits, labels) if labels is not None else None
+        loss = causal_lm_loss(logits, labels, packed) if labels is not None else None
         return {"loss": loss, "logits": logits, "past_key_values": presents}

@@ -21,8 +21,9 @@ from .fused_kernels_utils import (FusedBiasActivation, FusedBiasDropout, FusedBi
                                  FusedMergeHeads,
                                  FusedRotaryPositionEmbedding, FusedScaleMaskSoftmax,
                                  FusedScaleMaskSoftmaxDropout, FusedScaleMaskWindowSoftmax)
-from .modeling_utils import (ACT2FN, LayerPolicy, PreTrainedModel, StaticKV, additive_attention_mask, append_kv,
-                             causal_lm_loss, static_cache_mask)
+from .modeling_utils import (ACT2FN, LayerPolicy, PreTrainedModel, SequenceLayer, StaticKV, additive_attention_mask,
+                             append_kv, causal_lm_loss, packed_past, sequence_attention, sequence_positions,
+                             static_cache_mask)
 
 
 @dataclass
@@ -45,6 +46,10 @@ class GPTNeoConfig:
         if not self.attention_layers:
             self.attention_layers = ["global", "local"] * (self.num_layers // 2) + \
                                     ["global"] * (self.num_layers % 2)
+
+    @property
+    def num_attention_heads(self):
+        return self.num_heads
 
 
 class GPTNeoSelfAttention(nn.Module):
@@ -151,6 +156,13 @@ class FusedGPTNeoSelfAttention(GPTNeoSelfAttention):
                 use_cache=False, output_attentions=False, residual=None):
         """``residual``: added to the output (the residual connection of the
         block, which a decoding step takes into the projection's launch)."""
+        if isinstance(layer_past, SequenceLayer):
+            tokens = hidden_states.shape[1]
+            query, key, value = (t.view(tokens, self.num_heads, self.head_dim) for t in FusedLinearRows.project_many(
+                (self.q_proj, self.k_proj, self.v_proj), hidden_states))
+            out = sequence_attention(self, layer_past, query, key, value, 1.0, self._window(), head_mask, attention_mask,
+                                     output_attentions)
+            return self._output(out, residual), layer_past
         query, key, value, present = self._project_qkv(hidden_states, layer_past, use_cache)
         (bsz, np_, sq, _), sk = query.size(), key.size(-2)
         # a single query over a key/value cache (a decoding step) sees every key
@@ -191,6 +203,11 @@ class FusedGPTNeoSelfAttention(GPTNeoSelfAttention):
         else:
             out, w = self._attn(query, key, value, attention_mask, head_mask, causal=not static)
         out = FusedMergeHeads.apply(out) if self._transposes_fused(out) else self._merge_heads(out)
+        out = self._output(out, residual)
+        return (out, present, w) if output_attentions else (out, present)
+
+    def _output(self, out, residual):
+        """The output projection with its bias, dropout and the block's residual addition."""
         if FusedLinearRows.is_available(out, self.out_proj.weight) and not (
                 self.training and self.resid_dropout.p > 0.0):
             out = FusedLinearRows.apply(out, self.out_proj.weight, self.out_proj.bias, residual=residual)
@@ -201,7 +218,7 @@ class FusedGPTNeoSelfAttention(GPTNeoSelfAttention):
             else:  # bias, dropout and the block's residual addition in one pass
                 out = FusedBiasDropoutResidual.apply(out, self.out_proj.bias, residual, self.training,
                                                      self.resid_dropout.p)
-        return (out, present, w) if output_attentions else (out, present)
+        return out
 
 
 class FusedGPTNeoLocalSelfAttention(FusedGPTNeoSelfAttention, GPTNeoLocalSelfAttention):
@@ -298,6 +315,8 @@ class FusedGPTNeoBlock(GPTNeoBlock):
     (oslo/models/gpt_neo/configuration_gpt_neo.py:330-342); the arithmetic is
     that of oslo/models/gpt_neo/modeling_gpt_neo.py:333-380."""
 
+    takes_sequences = True
+
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         inner = self.attn.attention
         if not (isinstance(inner, FusedGPTNeoSelfAttention) and isinstance(self.mlp, FusedGPTNeoMLP)):
@@ -327,7 +346,10 @@ class GPTNeoModel(nn.Module):
         self.ln_f = nn.LayerNorm(config.hidden_size, eps=config.layer_norm_epsilon)
 
     def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False):
-        if past_key_values is not None and isinstance(past_key_values[0], StaticKV):
+        pos = sequence_positions(past_key_values, input_ids, self.wpe.num_embeddings, self.h)
+        if pos is not None:
+            pass  # sequences of different lengths
+        elif past_key_values is not None and isinstance(past_key_values[0], StaticKV):
             pos = past_key_values[0].state.pos
         else:
             past_len = 0 if past_key_values is None else past_key_values[0][0].size(-2)
@@ -355,9 +377,13 @@ class GPTNeoForCausalLM(PreTrainedModel):
     def get_layer_policies(self):
         return [GPTNeoLayerPolicy]
 
-    def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False, labels=None):
+    def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False, labels=None, packed=None):
+        """``packed``: a ``PackedSequences``: input_ids [1, tokens] are its sequences
+        one behind the other, none of which sees another (fused modules only)."""
+        if packed is not None:
+            past_key_values = packed_past(len(self.transformer.h), packed, past_key_values, attention_mask, use_cache)
         h, presents = self.transformer(input_ids, attention_mask, past_key_values, use_cache)
         fused_head = getattr(self, "fused_lm_head", False) and not self.training
         logits = FusedLinearRows.project(self.lm_head, h) if fused_head else self.lm_head(h)
-        loss = causal_lm_loss(logits, labels) if labels is not None else None
+        loss = causal_lm_loss(logits, labels, packed) if labels is not None else None
         return {"loss": loss, "logits": logits, "past_key_values": presents}

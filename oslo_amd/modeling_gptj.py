@@ -23,8 +23,9 @@ from .fused_kernels_utils import (FusedBiasActivation, FusedBiasDropout, FusedBi
                                  FusedMergeHeads,
                                  FusedRotaryPositionEmbedding,
                                  FusedScaleMaskSoftmax, FusedScaleMaskSoftmaxDropout)
-from .modeling_utils import (ACT2FN, LayerPolicy, PreTrainedModel, StaticKV, additive_attention_mask, append_kv,
-                             causal_lm_loss, static_cache_mask)
+from .modeling_utils import (ACT2FN, LayerPolicy, PreTrainedModel, SequenceLayer, StaticKV, additive_attention_mask,
+                             append_kv, causal_lm_loss, packed_past, sequence_attention, sequence_positions,
+                             static_cache_mask)
 
 
 @dataclass
@@ -77,7 +78,15 @@ def rotary_tables(dim, seq_len, device):
 def rotary_for_step(layer_past, dim, seq_len, device):
     """(sin, cos, offset) for ``seq_len`` new tokens after the cached ones. With
     a static cache the position lives on the device: the one table row of the
-    step is gathered there and the offset into it is 0."""
+    step is gathered there and the offset into it is 0; sequences of different
+    lengths take a row per token, that of its position in its own sequence."""
+    if isinstance(layer_past, SequenceLayer):
+        rows = layer_past.shared.get(("rotary", dim, seq_len))
+        if rows is None:  # the first layer of a forward gathers them, the others reuse them
+            sin, cos = rotary_tables(dim, max(layer_past.max_position, 1), device)
+            at = layer_past.row_positions(seq_len)
+            rows = layer_past.shared[("rotary", dim, seq_len)] = (sin.index_select(0, at), cos.index_select(0, at))
+        return rows[0], rows[1], 0
     if isinstance(layer_past, StaticKV):
         state = layer_past.state
         row = state.step_values.get(("rotary", dim))
@@ -180,15 +189,20 @@ class FusedGPTJAttention(GPTJAttention):
         if not (hidden_states.is_cuda and
                 FusedRotaryPositionEmbedding.is_available(hidden_states.dtype, self.head_dim, rot)):
             return super()._project_qkv(hidden_states, layer_past, use_cache)
+        query, key, value = self._project_rotated(hidden_states, layer_past)
+        key, value, present = append_kv(layer_past, key, value, use_cache, defer=True)
+        return query, key, value, present
+
+    def _project_rotated(self, hidden_states, layer_past):
+        """Rotated query and key, and value, [B, H, S, D]."""
+        rot = self.rotary_dim if self.rotary_dim is not None else self.head_dim
         b, s, _ = hidden_states.shape
         shape = (b, s, self.num_attention_heads, self.head_dim)
         sin, cos, offset = rotary_for_step(layer_past, rot, s, hidden_states.device)
         # (a decoding step streams the three weights in one launch)
         query, key, value = FusedLinearRows.project_many((self.q_proj, self.k_proj, self.v_proj), hidden_states)
-        query, key, value = FusedRotaryPositionEmbedding.apply(
+        return FusedRotaryPositionEmbedding.apply(
             query.view(shape), key.view(shape), value.view(shape), (sin, cos), rot, offset)
-        key, value, present = append_kv(layer_past, key, value, use_cache, defer=True)
-        return query, key, value, present
 
     def _fused_attn(self, query, key, value, attention_mask=None, head_mask=None, causal=True):
         w = torch.matmul(query, key.transpose(-1, -2))
@@ -204,6 +218,11 @@ class FusedGPTJAttention(GPTJAttention):
                 use_cache=False, output_attentions=False, residual=None):
         """``residual``: added to the output (the residual connection of the
         block, which a decoding step takes into the projection's launch)."""
+        if isinstance(layer_past, SequenceLayer):
+            query, key, value = (t[0].transpose(0, 1) for t in self._project_rotated(hidden_states, layer_past))
+            out = sequence_attention(self, layer_past, query, key, value, 1.0 / self.scale_attn, None, head_mask,
+                                     attention_mask, output_attentions)
+            return self._output(out, residual), layer_past
         query, key, value, present = self._project_qkv(hidden_states, layer_past, use_cache)
         (bsz, np_, sq, _), sk = query.size(), key.size(-2)
         # a single query over a key/value cache (a decoding step) sees every key:
@@ -237,10 +256,15 @@ class FusedGPTJAttention(GPTJAttention):
             out, w = self._fused_attn(query, key, value, attention_mask, head_mask, causal)
         else:
             out, w = self._attn(query, key, value, attention_mask, head_mask, causal=not static)
-        # out_proj has no bias: the epilogue kernel runs with the bias term
-        # dropped (in training; it is skipped when there is nothing to drop)
         vec_ok = FusedRotaryPositionEmbedding.is_available(out.dtype, self.head_dim, 0)
         out = FusedMergeHeads.apply(out) if out.is_cuda and vec_ok else self._merge_heads(out)
+        out = self._output(out, residual)
+        return (out, present, w) if output_attentions else (out, present)
+
+    def _output(self, out, residual):
+        """The output projection with dropout and the block's residual addition.
+        out_proj has no bias: the epilogue kernel runs with the bias term dropped
+        (in training; it is skipped when there is nothing to drop)."""
         if residual is not None and FusedLinearRows.is_available(out, self.out_proj.weight) and not (
                 self.training and self.resid_dropout.p > 0.0):
             out = FusedLinearRows.apply(out, self.out_proj.weight, residual=residual)  # a decoding step
@@ -250,7 +274,7 @@ class FusedGPTJAttention(GPTJAttention):
                 out = FusedBiasDropout.apply(out, None, self.training, self.resid_dropout.p)
             else:  # dropout and the block's residual addition in one pass
                 out = FusedBiasDropoutResidual.apply(out, None, residual, self.training, self.resid_dropout.p)
-        return (out, present, w) if output_attentions else (out, present)
+        return out
 
 
 class GPTJMLP(nn.Module):
@@ -328,6 +352,8 @@ class FusedGPTJBlock(GPTJBlock):
     feed-forward output on top). No counterpart in the reference, which fuses
     attention and MLP only (oslo/models/gptj/configuration_gptj.py:155-167)."""
 
+    takes_sequences = True
+
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         if not (isinstance(self.attn, FusedGPTJAttention) and isinstance(self.mlp, FusedGPTJMLP)):
             return super().forward(hidden_states, layer_past, attention_mask, head_mask, use_cache)
@@ -358,6 +384,7 @@ class GPTJModel(nn.Module):
         self.ln_f = nn.LayerNorm(config.n_embd, eps=config.layer_norm_epsilon)
 
     def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False):
+        sequence_positions(past_key_values, input_ids, None, self.h)  # (for its checks: angles know no last position)
         h = self.drop(self.wte(input_ids))
         mask = additive_attention_mask(attention_mask, h.dtype)
         presents = []
@@ -380,9 +407,13 @@ class GPTJForCausalLM(PreTrainedModel):
     def get_layer_policies(self):
         return [GPTJLayerPolicy]
 
-    def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False, labels=None):
+    def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False, labels=None, packed=None):
+        """``packed``: a ``PackedSequences``: input_ids [1, tokens] are its sequences
+        one behind the other, none of which sees another (fused modules only)."""
+        if packed is not None:
+            past_key_values = packed_past(len(self.transformer.h), packed, past_key_values, attention_mask, use_cache)
         h, presents = self.transformer(input_ids, attention_mask, past_key_values, use_cache)
         fused_head = getattr(self, "fused_lm_head", False) and not self.training
         logits = FusedLinearRows.project(self.lm_head, h) if fused_head else self.lm_head(h)
-        loss = causal_lm_loss(logits, labels) if labels is not None else None
+        loss = causal_lm_loss(logits, labels, packed) if labels is not None else None
         return {"loss": loss, "logits": logits, "past_key_values": presents}

@@ -15,6 +15,7 @@ from torch import nn
 
 from .fused_kernels_utils import FusedKernelMixin
 from .generation_utils import GenerationMixin
+from .sequences import SequenceLayer, packed_labels, sequence_layers
 
 
 class Conv1D(nn.Module):
@@ -228,7 +229,45 @@ def additive_attention_mask(attention_mask, dtype):
     return (1.0 - m) * -10000.0
 
 
-def causal_lm_loss(logits, labels):
+def sequence_attention(module, layer_past, query, key, value, scale, window, head_mask, attention_mask,
+                       output_attentions):
+    """The attention of a fused module over sequences of different lengths:
+    query, key, value [T, heads, D] -> [1, T, heads * D]."""
+    if head_mask is not None or attention_mask is not None or output_attentions:
+        raise RuntimeError("packed and paged attention take no masks and return no probabilities")
+    if module.training and module.attn_dropout.p > 0.0:
+        raise RuntimeError("packed attention does not drop probabilities: set the attention dropout to 0")
+    out = layer_past.attend(query, key, value, scale, window)
+    return out.reshape(1, out.shape[0], -1)
+
+
+def packed_past(model_layers, packed, past_key_values, attention_mask, use_cache):
+    """``past_key_values`` of a forward with ``packed``: one layer object per block."""
+    if past_key_values is not None or attention_mask is not None or use_cache:
+        raise ValueError("packed sequences come without past_key_values, attention_mask and use_cache")
+    return sequence_layers(packed, model_layers)
+
+
+def sequence_positions(past_key_values, input_ids, limit, blocks):
+    """Positions of the tokens when ``past_key_values`` are ``SequenceLayer``s,
+    else None. The unfused modules do not know them. ``limit``: the positions the
+    model knows (None: any)."""
+    if past_key_values is None or not isinstance(past_key_values[0], SequenceLayer):
+        return None
+    if not hasattr(blocks[0], "takes_sequences"):
+        raise RuntimeError("sequences of different lengths need the fused modules: call model.fuse() first")
+    if input_ids.dim() != 2 or input_ids.size(0) != 1:
+        raise ValueError("sequences of different lengths are one row of tokens: input_ids must be [1, tokens]")
+    layer = past_key_values[0]
+    if limit is not None and layer.max_position > limit:
+        raise ValueError(f"sequences of up to {layer.max_position} positions; the model has {limit}")
+    return layer.row_positions(input_ids.size(1))
+
+
+def causal_lm_loss(logits, labels, packed=None):
+    if packed is not None:
+        targets = packed_labels(labels, packed)
+        return nn.functional.cross_entropy(logits.view(-1, logits.size(-1)).float(), targets.view(-1))
     shift_logits = logits[..., :-1, :].contiguous()
     shift_labels = labels[..., 1:].contiguous()
     return nn.functional.cross_entropy(shift_logits.view(-1, shift_logits.size(-1)).float(),

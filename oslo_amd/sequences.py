@@ -7,6 +7,8 @@ and whose cache grows by concatenation
 import numpy as np
 import torch
 
+from .fused_kernels_utils import FusedPackedAttention, FusedPagedDecodeAttention, FusedPagedKV
+
 PACKED_BLOCK = 128  # positions of a sequence one block of the attention kernels takes
 CUS = 256  # of an MI355X
 
@@ -145,3 +147,106 @@ class PagedKV(object):
         pages = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
         scales = [torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2)]
         return cls(*pages, table, *scales)
+
+
+class SequenceLayer(object):
+    """What a fused attention module is handed as ``layer_past`` when its tokens
+    [1, T] belong to sequences of different lengths: ``attend`` takes query
+    [T, H, D], key and value [T, Hkv, D] and returns [T, H, D]; ``positions``
+    (int32 on the device) are the tokens' positions in their sequences, all
+    below ``max_position``; ``shared`` holds what the layers of one forward
+    work out once."""
+
+    positions = max_position = shared = None
+
+    def row_positions(self, tokens):
+        """``positions`` for a row of ``tokens``: 0 behind the last sequence (such
+        rows are computed and seen by nobody)."""
+        extra = tokens - self.positions.numel()
+        if extra < 0:
+            raise ValueError(f"{self.positions.numel()} tokens of sequences in a row of {tokens}")
+        return torch.cat([self.positions, self.positions.new_zeros(extra)]) if extra else self.positions
+
+    def attend(self, query, key, value, scale, window=None):
+        raise NotImplementedError
+
+
+class PackedLayer(SequenceLayer):
+    """Whole sequences packed into the row (prompts or training documents);
+    with ``cache`` their keys and values also go into that layer's ``PagedKV``."""
+
+    def __init__(self, packed, cache, shared):
+        self.packed, self.cache, self.shared = packed, cache, shared
+        self.positions, self.max_position = packed.positions, packed.max_length
+
+    def attend(self, query, key, value, scale, window=None):
+        if self.cache is not None:
+            n = self.packed.total
+            FusedPagedKV.write(self.cache, key[:n], value[:n], self.packed.sequence, self.packed.positions)
+        return FusedPackedAttention.apply(query, key, value, self.packed, scale, window)
+
+
+class PagedState(object):
+    """The layers' paged caches while one token per sequence is decoded at a
+    time, under one table, with pages for ``capacity`` positions of each sequence.
+    ``lengths`` (int32 [sequences] on the device) counts the positions written,
+    which is also the position of the token being fed: nothing in a step depends
+    on the host, so a step can be captured into a graph and replayed."""
+
+    def __init__(self, lengths, capacity, layers, kv_heads, head_dim, dtype, device, page_size=64, quantized=False):
+        self.capacity = int(capacity)
+        if self.capacity < 1 or any(not 0 <= n <= self.capacity for n in lengths):
+            raise ValueError("PagedState: lengths from zero to a capacity of at least one position")
+        each = -(-self.capacity // page_size)
+        num_pages = len(lengths) * each
+        self.table = torch.arange(num_pages, dtype=torch.int32, device=device).view(len(lengths), each)
+        self.lengths = torch.tensor([int(n) for n in lengths], dtype=torch.int32, device=device)
+        self.visible = self.lengths + 1
+        self.rows = torch.arange(len(lengths), dtype=torch.int32, device=device)
+        self.step_values = {}  # what layers share within one step
+        self.caches = [PagedKV.allocate(self.table, num_pages, kv_heads, page_size, head_dim, dtype, device, quantized)
+                       for _ in range(layers)]
+
+    def prompt_layers(self, packed):
+        """``layer_past`` of every layer for the prompts, packed into one row."""
+        shared = {}
+        return [PackedLayer(packed, cache, shared) for cache in self.caches]
+
+    def begin_step(self):
+        """``layer_past`` of every layer for the next tokens, [1, sequences]."""
+        self.step_values.clear()
+        torch.add(self.lengths, 1, out=self.visible)
+        return [PagedLayer(self, cache) for cache in self.caches]
+
+    def end_step(self):
+        """The tokens are in the cache. A sequence that is full stays at its last
+        position, which its next tokens overwrite."""
+        self.lengths.add_(1).clamp_(max=self.capacity - 1)
+
+
+class PagedLayer(SequenceLayer):
+    """One new token per sequence over a layer's paged cache."""
+
+    def __init__(self, state, cache):
+        self.state, self.cache, self.shared = state, cache, state.step_values
+        self.positions, self.max_position = state.lengths, state.capacity
+
+    def attend(self, query, key, value, scale, window=None):
+        FusedPagedKV.write(self.cache, key, value, self.state.rows, self.state.lengths)
+        return FusedPagedDecodeAttention.apply(query, self.cache, self.state.visible, scale, window)
+
+
+def sequence_layers(packed, layers):
+    """``layer_past`` of every layer for tokens packed into one row."""
+    shared = {}
+    return [PackedLayer(packed, None, shared) for _ in range(layers)]
+
+
+def packed_labels(labels, packed):
+    """Targets of a packed row: the next token of the same sequence; -100 (no
+    target) at a sequence's last token and behind the last sequence."""
+    targets = torch.full_like(labels, -100)
+    if packed.total > 1:
+        first = packed.positions[1:] == 0
+        targets[..., :packed.total - 1] = labels[..., 1:packed.total].masked_fill(first, -100)
+    return targets

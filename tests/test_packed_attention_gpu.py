@@ -83,6 +83,18 @@ CASES = [([1], 2, 2, 64, 0), ([1, 1, 1], 4, 2, 128, 0), ([0, 5, 0, 128, 129, 127
          ([400, 130, 1], 8, 2, 128, 1), ([700, 65], 5, 5, 64, 256), ([1100], 12, 12, 64, 300), ([260, 260], 16, 2, 128, 259)]
 
 
+# one long sequence, few key/value heads: the longest dK/dV walks are shared over a group's heads
+SHARED = [([2000], 8, 1, 128, 0), ([1500, 3], 16, 2, 256, 0), ([1700, 200], 12, 1, 64, 0), ([2100], 8, 2, 128, 1500)]
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=IDS.get)
+@pytest.mark.parametrize("lengths,heads,kv_heads,d,window", SHARED, ids=lambda v: str(v).replace(" ", ""))
+def test_gradients_of_shared_walks(lengths, heads, kv_heads, d, window, dtype):
+    split, parts = PackedSequences(lengths, "cpu").shared_blocks(heads, kv_heads, d, window)
+    assert split > 0 and parts > 1
+    test_output_and_gradients(lengths, heads, kv_heads, d, window, dtype)
+
+
 @pytest.mark.parametrize("dtype", HALVES, ids=IDS.get)
 @pytest.mark.parametrize("lengths,heads,kv_heads,d,window", CASES, ids=lambda v: str(v).replace(" ", ""))
 def test_output_and_gradients(lengths, heads, kv_heads, d, window, dtype):
@@ -268,3 +280,31 @@ def test_list_entries_out_of_range_are_passed_over():
     packed.blocks = torch.tensor([[[0, 20, 0, 0], [-1, 4, 0, 0], [25, 6, 0, 0], [0, 20, 1, 0], [0, 0, 0, 0],
                                    [0, 21, 0, 0], [3, 4, -1, 0]]] * 2, dtype=torch.int32, device=DEV)
     assert torch.equal(kernels.attention_packed_forward(q, k, v, packed, 0.1), want)
+
+
+def test_a_capture_is_refused_while_an_eager_graph_of_the_same_leaf_lives():
+    packed = PackedSequences([40], DEV)
+    q, k, v = (torch.randn(40, 2, 64, device=DEV, dtype=torch.float16, requires_grad=True) for _ in range(3))
+    grad = torch.ones(40, 2, 64, device=DEV, dtype=torch.float16)
+    living = FusedPackedAttention.apply(q, k, v, packed)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph):
+            FusedPackedAttention.apply(q, k, v, packed)
+    torch.autograd.backward(living, grad)
+    want = [t.grad.clone() for t in (q, k, v)]
+    del living
+    for t in (q, k, v):
+        t.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = FusedPackedAttention.apply(q, k, v, packed)
+        torch.autograd.backward(out, grad)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for t, w in zip((q, k, v), want):
+            assert torch.equal(t.grad, w)
+            t.grad.zero_()

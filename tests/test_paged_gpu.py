@@ -208,6 +208,27 @@ def test_decode_attention(lengths, heads, kv_heads, d, page, window, eight, dtyp
         assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("eight", [False, True], ids=["16bit", "8bit"])
+@pytest.mark.parametrize("count,longest,window", [(64, 200, 0), (65, 300, 0), (300, 150, 40), (4097, 40, 0), (9000, 33, 5)])
+def test_decode_of_many_sequences(count, longest, window, eight):
+    """Numbers of sequences around those that one wave, one block and one pass of the chunks' list take."""
+    heads, kv_heads, d, page, dtype = 2, 1, 64, 16, torch.bfloat16
+    lengths = torch.randint(0, longest + 1, (count,), generator=torch.Generator().manual_seed(count)).tolist()
+    cache, keys, values = filled(lengths, kv_heads, d, page, dtype, eight, seed=count)
+    q = randn((count, heads, d), dtype, seed=7).to(DEV)
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    out = FusedPagedDecodeAttention.apply(q, cache, n, 0.125, window or None)
+    k, v = (torch.nn.utils.rnn.pad_sequence(x, batch_first=True)[:, :, 0].double() for x in (keys, values))
+    at = torch.arange(k.shape[1], device=DEV)[None, :]
+    hidden = (at >= n[:, None]) | ((at < n[:, None] - window) if window else torch.zeros_like(at, dtype=torch.bool))
+    s = (q.double() @ k.transpose(1, 2) * 0.125).masked_fill(hidden[:, None], -math.inf)
+    p = torch.softmax(s, -1).nan_to_num(0.0)  # (a sequence of nothing)
+    want, mag = p @ v, p @ v.abs()
+    assert torch.isfinite(out).all()
+    assert ((out.double() - want).abs() <= 1.05 * REL[dtype] * (want.abs() + mag) + 2.0 ** -15 * mag + 1e-7).all()
+    assert not out[n == 0].any()
+
+
 def test_decode_scores_far_apart():
     """A maximum that keeps rising by more than an exponential can hold, and one key that outweighs the rest."""
     n, d = 500, 64

@@ -8,8 +8,9 @@ import numpy as np
 import pytest
 import torch
 
-from oslo_amd import PackedSequences, PagedKV, kernels
+from oslo_amd import GPT2Config, GPT2LMHeadModel, PackedSequences, PagedKV, PagedState, kernels
 from oslo_amd import _lib
+from oslo_amd.sequences import packed_labels, sequence_layers
 
 
 @pytest.mark.parametrize("lengths", [[], [0], [1], [0, 5, 0, 128, 129, 127, 0], [300, 31, 33, 64, 1000]],
@@ -177,3 +178,71 @@ def test_entry_points_screen_their_arguments():
     assert sample(vocab=0) == -1 and sample(vocab=2 ** 24 + 1) == -2 and sample(rows=-1) == -1
     assert sample(dtype=5) == -1 and sample(tokens=null) == -1 and sample(logits=null) == -1
     assert sample(rows=0) == 0
+
+
+def test_labels_of_a_packed_row_stay_inside_their_sequences():
+    """Next tokens; none at a sequence's end, behind the last sequence, or where the caller has none."""
+    packed = PackedSequences([3, 0, 1, 4], "cpu")
+    labels = torch.tensor([[10, 11, 12, 20, 30, 31, -100, 33, 98, 99]])
+    assert packed_labels(labels, packed).tolist() == [[11, 12, -100, -100, 31, -100, 33, -100, -100, -100]]
+    assert packed_labels(labels[:, :1], PackedSequences([1], "cpu")).tolist() == [[-100]]
+    assert packed_labels(labels[:, :0], PackedSequences([], "cpu")).tolist() == [[]]
+
+
+def test_positions_of_a_row_with_tokens_behind_the_last_sequence():
+    layer = sequence_layers(PackedSequences([2, 3], "cpu"), 1)[0]
+    assert layer.row_positions(5).tolist() == [0, 1, 0, 1, 2]
+    assert layer.row_positions(7).tolist() == [0, 1, 0, 1, 2, 0, 0]
+    with pytest.raises(ValueError, match="5 tokens of sequences in a row of 4"):
+        layer.row_positions(4)
+
+
+def test_paged_state_gives_every_sequence_its_own_pages_and_stops_at_the_last_position():
+    state = PagedState([3, 130, 0], 131, 2, 2, 64, torch.float16, "cpu")
+    assert state.table.shape == (3, 3) and sorted(state.table.flatten().tolist()) == list(range(9))
+    assert len(state.caches) == 2 and all(c.key_pages.shape == (9, 2, 64, 64) for c in state.caches)
+    layers = state.begin_step()
+    assert state.visible.tolist() == [4, 131, 1] and layers[1].positions is state.lengths
+    state.end_step()
+    assert state.lengths.tolist() == [4, 130, 1]
+    for bad in (dict(lengths=[5], capacity=4), dict(lengths=[-1], capacity=4), dict(lengths=[0], capacity=0)):
+        with pytest.raises(ValueError, match="PagedState"):
+            PagedState(**bad, layers=1, kv_heads=1, head_dim=64, dtype=torch.float16, device="cpu")
+
+
+def test_models_refuse_what_sequences_do_not_take():
+    model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
+    row, packed = torch.zeros((1, 6), dtype=torch.long), PackedSequences([2, 4], "cpu")
+    with pytest.raises(RuntimeError, match="fuse"):
+        model(row, packed=packed)
+    with pytest.raises(ValueError, match="without past_key_values"):
+        model(row, packed=packed, use_cache=True)
+    with pytest.raises(ValueError, match="without past_key_values"):
+        model(row, packed=packed, attention_mask=torch.ones_like(row))
+    model.fuse()
+    with pytest.raises(ValueError, match="one row"):
+        model(row.view(2, 3), packed=packed)
+    with pytest.raises(ValueError, match="the model has 8"):
+        model(torch.zeros((1, 9), dtype=torch.long), packed=PackedSequences([9], "cpu"))
+    with pytest.raises(ValueError, match="6 tokens of sequences in a row of 5"):
+        model(row[:, :5], packed=packed)
+    with pytest.raises(RuntimeError, match="drop"):
+        model.train()(row, packed=packed)
+
+
+def test_generate_refuses_what_sampling_and_lists_do_not_take():
+    model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
+    ids = torch.zeros((1, 3), dtype=torch.long)
+    with pytest.raises(ValueError, match="num_beams=1"):
+        model.generate(ids, max_length=5, do_sample=True, num_beams=2)
+    with pytest.raises(ValueError, match="list of prompts"):
+        model.generate(ids, max_length=5, quantized_cache=True)
+    for kw in (dict(num_beams=2), dict(no_repeat_ngram_size=2), dict(static_cache=True), dict(use_cache=False)):
+        with pytest.raises(ValueError, match="its own paged cache"):
+            model.generate([ids[0]], max_length=5, **kw)
+    for bad in ([ids], [ids[0, :0]], [ids[0].repeat(2)]):
+        with pytest.raises(ValueError, match="1-D tensors of 1 to max_length - 1 = 4"):
+            model.generate(bad, max_length=5)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        model.generate([ids[0]], max_length=5)
+    assert model.generate([], max_length=5) == []
