@@ -12,8 +12,8 @@
 //
 // Which token comes out is a whole number, so a border of the filters or of the
 // draw must not move with the order of a sum. Masses are therefore whole numbers
-// too: exp in 64 bits, times 2^S, rounded (S = 62 - ceil(log2 vocabulary), 46 at
-// fifty thousand tokens; a rounding of 2^-47 of the largest mass, ten million
+// too: exp in 64 bits, times 2^S, rounded (S = 61 - ceil(log2 vocabulary), at most 49; 45 at
+// fifty thousand tokens; a rounding of 2^-46 of the largest mass, ten million
 // times finer than a 32-bit sum). Sums of whole numbers are exact in any order:
 // histograms may use atomics and every run gives the same token.
 //
@@ -40,9 +40,8 @@
 namespace oslo {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kBins = 2048;
+constexpr int kMostWaves = 16;
 
 typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
@@ -75,11 +74,12 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// 2^(i / 1024), i = 0 .. 1023, by the Taylor series of e^(i / 1024 ln 2) (to the
+// 2^((i - 1/2) / 1024), i = 0 .. 1023, by the Taylor series of the exponential (to the
 // eighteenth power: below 2^-60 of the result); once per block.
 constexpr int kTable = 1024;
+constexpr double kStep = 0.69314718055994530942 / kTable; // of the natural logarithm between two entries
 __device__ __forceinline__ double table_entry(int i) {
-  const double z = (double)i * (0.69314718055994530942 / kTable);
+  const double z = ((double)i - 0.5) * kStep;
   double s = 1.0;
 #pragma unroll
   for (int n = 18; n >= 1; --n) s = __builtin_fma(s * z, 1.0 / n, 1.0);
@@ -91,24 +91,22 @@ __device__ __forceinline__ float next_below(float x) {
   if (x == -INFINITY) return x;
   return key_value((x == 0.f ? 0x7fffffffu : order_key(x)) - 1); // (0 and -0 are one number)
 }
-__device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) {
-  const uint32_t lo = __shfl_up((uint32_t)v, d, kWave), hi = __shfl_up((uint32_t)(v >> 32), d, kWave);
-  return (u64)hi << 32 | lo;
-}
-// Sum over the lanes up to and including this one.
-__device__ __forceinline__ u64 wave_scan_u64(u64 v, int lane) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const u64 w = shfl_up_u64(v, d);
-    if (lane >= d) v += w;
-  }
-  return v;
-}
-template <int CTRL>
+template <int CTRL, int ROWS = 0xf>
 __device__ __forceinline__ u64 dpp_u64(u64 v) { // (lanes that receive nothing get 0)
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xf, 0xf, true);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xf, 0xf, true);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, true);
   return (u64)hi << 32 | lo;
+}
+// Sum over the lanes up to and including this one: within rows of 16 by shifts of 1, 2,
+// 4 and 8, then the last lane of a row to the next row, and lane 31 to the upper half.
+__device__ __forceinline__ u64 wave_scan_u64(u64 v) {
+  v += dpp_u64<0x111>(v);
+  v += dpp_u64<0x112>(v);
+  v += dpp_u64<0x114>(v);
+  v += dpp_u64<0x118>(v);
+  v += dpp_u64<0x142, 0xa>(v);
+  v += dpp_u64<0x143, 0xc>(v);
+  return v;
 }
 // Sum over the wave, for every lane: rows of 16 on the vector ALU, the four rows by lane reads.
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
@@ -129,15 +127,18 @@ constexpr int kRanked = 512;  // ... of which so many are ranked by counting
 
 struct alignas(16) SampleLds {
   u64 bins[kBins];
-  u64 segments[kBins];
-  u64 list[kListed]; // order_key(logit) << 32 | ~index: distinct, and in the filters' order
-  u64 ranked[kRanked];
+  union {
+    u64 list[kListed]; // order_key(logit) << 32 | ~index: distinct, and in the filters' order
+    uint32_t counts[kBins + kWave];
+  };
+  u64 picked[kRanked], ranked[kRanked];
   double table[kTable];
-  u64 wave_sums[kWaves];
-  float wave_max[kWaves], wave_min[kWaves];
+  u64 wave_sums[kMostWaves], wave_all[kMostWaves], wave_kept[kMostWaves];
+  float wave_max[kMostWaves], wave_min[kMostWaves];
   u64 found_before, found_value; // results of a search, written by the one thread that finds them
-  int found_at;
-  int listed;
+  double log_total;
+  int found_at, found_too;
+  int listed, num_picked;
   uint32_t bound;
 };
 __device__ __forceinline__ u64 list_entry(float x, int index) {
@@ -146,19 +147,22 @@ __device__ __forceinline__ u64 list_entry(float x, int index) {
 __device__ __forceinline__ float entry_logit(u64 e) { return key_value((uint32_t)(e >> 32)); }
 __device__ __forceinline__ int entry_index(u64 e) { return (int)~(uint32_t)e; }
 
-// A running sum over bins[0 .. kBins): each thread's share (consecutive bins), what
-// lies before it, and the total. The bins must be complete (a barrier has passed).
-constexpr int kBinsEach = kBins / kThreads;
+// A running sum over kBins values: each thread's share (consecutive ones), what lies
+// before it, and the total.
+template <int kThreads>
 struct BinScan {
-  u64 before, mine, total;
+  static constexpr int kEach = kBins / kThreads;
+  u64 v[kEach], before, mine, total;
+  __device__ __forceinline__ static int bin(int i) { return (int)threadIdx.x * kEach + i; }
 };
-__device__ __forceinline__ BinScan scan_bins(SampleLds &lds, const u64 *bins) {
+template <int kThreads>
+__device__ __forceinline__ BinScan<kThreads> scan_values(SampleLds &lds, BinScan<kThreads> s) {
+  constexpr int kBinsEach = s.kEach, kWaves = kThreads / kWave;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  BinScan s;
   s.mine = 0;
 #pragma unroll
-  for (int i = 0; i < kBinsEach; ++i) s.mine += bins[tid * kBinsEach + i];
-  const u64 upto = wave_scan_u64(s.mine, lane);
+  for (int i = 0; i < kBinsEach; ++i) s.mine += s.v[i];
+  const u64 upto = wave_scan_u64(s.mine);
   if (lane == kWave - 1) lds.wave_sums[wave] = upto;
   __syncthreads();
   s.before = upto - s.mine;
@@ -171,27 +175,39 @@ __device__ __forceinline__ BinScan scan_bins(SampleLds &lds, const u64 *bins) {
   }
   return s;
 }
-// The first bin at which the running sum reaches `target` (0 < target <= total), the
-// sum before it and its own value, for every thread.
+// The bins must be complete (a barrier has passed).
+template <int kThreads>
+__device__ __forceinline__ BinScan<kThreads> scan_bins(SampleLds &lds) {
+  BinScan<kThreads> s;
+#pragma unroll
+  for (int i = 0; i < s.kEach; ++i) s.v[i] = lds.bins[s.bin(i)];
+  return scan_values(lds, s);
+}
+// f(bin, sum before it, its value) for the first bin at which the running sum reaches
+// `target` (0 < target <= total), by the one thread that has it.
+template <int kThreads, typename F>
+__device__ __forceinline__ void at_target(const BinScan<kThreads> &s, u64 target, F &&f) {
+  u64 run = s.before;
+  if (run < target && run + s.mine >= target) {
+#pragma unroll
+    for (int i = 0; i < s.kEach; ++i) {
+      if (run < target && run + s.v[i] >= target) f(s.bin(i), run, s.v[i]);
+      run += s.v[i];
+    }
+  }
+}
+// The same, for every thread.
 struct Found {
   int at;
   u64 before, value;
 };
-__device__ __forceinline__ int tid_bin(int i) { return (int)threadIdx.x * kBinsEach + i; }
-__device__ __forceinline__ Found find_bin(SampleLds &lds, const u64 *bins, const BinScan &s, u64 target) {
-  u64 run = s.before;
-  if (run < target && run + s.mine >= target) { // exactly one thread
-#pragma unroll
-    for (int i = 0; i < kBinsEach; ++i) {
-      const u64 v = bins[tid_bin(i)];
-      if (run < target && run + v >= target) {
-        lds.found_at = tid_bin(i);
-        lds.found_before = run;
-        lds.found_value = v;
-      }
-      run += v;
-    }
-  }
+template <int kThreads>
+__device__ __forceinline__ Found find_bin(SampleLds &lds, const BinScan<kThreads> &s, u64 target) {
+  at_target(s, target, [&](int at, u64 before, u64 value) __attribute__((always_inline)) {
+    lds.found_at = at;
+    lds.found_before = before;
+    lds.found_value = value;
+  });
   __syncthreads();
   Found f;
   f.at = lds.found_at, f.before = lds.found_before, f.value = lds.found_value;
@@ -199,14 +215,16 @@ __device__ __forceinline__ Found find_bin(SampleLds &lds, const u64 *bins, const
   return f;
 }
 
-// Chunks (1024 threads x 16 bytes) of a row that the registers hold, and the most
-// that LDS holds behind them (with the tables above, 157 of a CU's 160 KiB).
-constexpr int kInRegisters = 7, kMostInLds = 6;
+// A row is cut into pieces of 16 bytes, and each wave takes a run of them, chunk by
+// chunk of 64. Chunks that the registers hold, and the most that LDS holds behind
+// them (with the tables above, 145 of a CU's 160 KiB).
+constexpr int kInRegisters = 7;
+constexpr int most_in_lds(int threads) { return threads == 1024 ? 6 : 3; }
 
-template <typename T>
+template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a) {
+  constexpr int kWaves = kThreads / kWave, kMostInLds = most_in_lds(kThreads), kBinsEach = kBins / kThreads;
   constexpr int kVec = Io<T>::kVec; // logits of a 16-byte load
-  constexpr int kChunk = kThreads * kVec;
   using V = RawVec<T, kVec>;
   extern __shared__ __align__(16) unsigned char lds_raw[];
   SampleLds &lds = *reinterpret_cast<SampleLds *>(lds_raw);
@@ -221,79 +239,81 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
   const int lead = (int)((reinterpret_cast<uintptr_t>(logits) & 15u) / sizeof(T));
   const V *const pieces = reinterpret_cast<const V *>(logits - lead);
   const int last_piece = (vocab + lead - 1) / kVec;
-  const int chunks = last_piece / kThreads + 1;
+  const int chunks = last_piece / kThreads + 1; // ... of a wave
   const T kNothing = static_cast<T>(-INFINITY);
   bool infinite = false; // the largest logit is +inf: only those count, as zeros among -inf
-  // index of the first logit of the vector that thread `t` of the block holds of chunk c (may be negative)
-  auto first_of = [&](int c, int t) __attribute__((always_inline)) { return c * kChunk + t * kVec - lead; };
-  auto load_raw = [&](int c, int t) __attribute__((always_inline)) {
-    const int piece = c * kThreads + t;
+  // the piece that lane `l` of this wave holds of chunk c, and the index of its first logit (may be negative)
+  auto piece_of = [&](int c, int l) __attribute__((always_inline)) { return (wave * chunks + c) * kWave + l; };
+  auto first_in = [&](int piece) __attribute__((always_inline)) { return piece * kVec - lead; };
+  auto first_of = [&](int c, int l) __attribute__((always_inline)) { return first_in(piece_of(c, l)); };
+  auto load_raw = [&](int piece) __attribute__((always_inline)) {
     return pieces[piece < last_piece ? piece : last_piece]; // (no branch: the loads of a thread are issued together)
   };
   // Beside the row: -inf. NaN becomes -inf, -0 becomes 0 (they are equal logits).
-  auto clean = [&](V &v, int c, int t) __attribute__((always_inline)) {
+  auto clean = [&](V &v, int piece) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const float x = static_cast<float>(v[e]) + 0.f;
-      const bool inside = (unsigned)(first_of(c, t) + e) < (unsigned)vocab;
-      v[e] = inside && x == x ? static_cast<T>(x) : kNothing;
-    }
+    for (int e = 0; e < kVec; ++e) v[e] = static_cast<T>(fmaxf(static_cast<float>(v[e]) + 0.f, -INFINITY));
+    const int first = __builtin_amdgcn_readfirstlane(piece); // (the wave's pieces lie one behind the other)
+    if (first == 0 || first + kWave > last_piece)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = (unsigned)(first_in(piece) + e) < (unsigned)vocab ? v[e] : kNothing;
   };
   auto only_infinite = [&](V &v) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) v[e] = static_cast<float>(v[e]) == INFINITY ? static_cast<T>(0.f) : kNothing;
   };
-  auto load = [&](int c, int t) __attribute__((always_inline)) {
-    V v = load_raw(c, t);
-    clean(v, c, t);
+  auto load = [&](int piece) __attribute__((always_inline)) {
+    V v = load_raw(piece);
+    clean(v, piece);
     if (infinite) only_infinite(v);
     return v;
   };
   V held[kInRegisters];
   const int in_lds = chunks - kInRegisters < kMostInLds ? chunks - kInRegisters : kMostInLds;
 #pragma unroll
-  for (int c = 0; c < kInRegisters; ++c) held[c] = load_raw(c, tid);
+  for (int c = 0; c < kInRegisters; ++c) held[c] = load_raw(piece_of(c, lane));
   if (in_lds > 0) {
     V more[kMostInLds];
 #pragma unroll
-    for (int c = 0; c < kMostInLds; ++c) more[c] = load_raw(kInRegisters + c, tid);
+    for (int c = 0; c < kMostInLds; ++c) more[c] = load_raw(piece_of(kInRegisters + c, lane));
 #pragma unroll
     for (int c = 0; c < kMostInLds; ++c)
       if (c < in_lds) {
-        clean(more[c], kInRegisters + c, tid);
+        clean(more[c], piece_of(kInRegisters + c, lane));
         lds_held[c * kThreads + tid] = more[c];
       }
   }
 #pragma unroll
-  for (int c = 0; c < kInRegisters; ++c) clean(held[c], c, tid);
-  lds.table[tid] = table_entry(tid); // (as many entries as threads)
+  for (int c = 0; c < kInRegisters; ++c) clean(held[c], piece_of(c, lane));
+#pragma unroll 1
+  for (int i = tid; i < kTable; i += kThreads) lds.table[i] = table_entry(i);
   // f(chunk, vector) for every vector of this thread. The empty statement "changes"
   // the vector: without it the compiler works out ahead, for all chunks at once, what
   // several passes have in common (conversions, whole masses, indices), and spills it.
-  int at_tid = tid; // the thread, for the indices of the vector being visited
+  int at_lane = lane; // the lane, for the indices of the vector being visited
   auto for_chunks = [&](auto &&f) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < kInRegisters; ++c)
       if (c < chunks) {
         u32x4_t w = __builtin_bit_cast(u32x4_t, held[c]);
-        at_tid = tid;
-        asm volatile("" : "+v"(w), "+v"(at_tid));
+        at_lane = lane;
+        asm volatile("" : "+v"(w), "+v"(at_lane));
         f(c, __builtin_bit_cast(V, w));
         __builtin_amdgcn_sched_barrier(0);
       }
-    at_tid = tid;
+    at_lane = lane;
 #pragma unroll 1
     for (int c = kInRegisters; c < chunks; ++c) {
       V v;
       if (c < kInRegisters + kMostInLds) v = lds_held[(c - kInRegisters) * kThreads + tid];
-      else v = load(c, tid);
+      else v = load(piece_of(c, lane));
       f(c, v);
     }
   };
   // the same, all of it read again (for searches that hardly ever run: little code)
   auto for_chunks_again = [&](auto &&f) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (int c = 0; c < chunks; ++c) f(c, load(c, tid));
+    for (int c = 0; c < chunks; ++c) f(c, load(piece_of(c, lane)));
   };
 
   // the largest logit of the thread, then of the row
@@ -333,7 +353,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
       for_chunks_again([&](int c, const V &v) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < kVec; ++e)
-          if (static_cast<float>(v[e]) == top) atomicMin(&lds.found_at, first_of(c, tid) + e);
+          if (static_cast<float>(v[e]) == top) atomicMin(&lds.found_at, first_of(c, lane) + e);
       });
     __syncthreads();
     if (tid == 0) {
@@ -344,22 +364,43 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
   }
 
   // Mass of a logit relative to the largest one's, as a whole number of 2^-S: with
-  // y = (x - top) * log2(e) / temperature = n / 1024 + r, |r| <= 2^-11, it is 2^(n / 1024)
-  // from the table times the series of 2^r = e^(r ln 2) to the third power (the next
-  // term is below 2^-50). The result times 2^S is below 2^52: adding 2^52 leaves the
-  // rounded whole number in the low bits.
+  // z = 1024 log2(e) (top - x) / temperature = n + r, 0 <= r < 1, it is 2^(-n / 1024)
+  // from the table times e^-(r kStep), a polynomial of the third power about r = 1/2 (the
+  // next term is below 2^-50). The result times 2^S is below 2^52: adding 2^52 rounds it to a
+  // whole number, in the low bits.
   const double per_unit = 1.4426950408889634074 / temperature;
+  const double per_entry = per_unit * kTable;
+  constexpr double kRounding = 4503599627370496.0;
+  constexpr u64 kMassBits = 0xfffffffffffffull;
+  // Of several logits at once, so that one's table read and its chain of 64-bit
+  // operations hide behind the others': w[i] = mass + 2^52.
+  auto rounded_masses = [&]<int N>(const float (&x)[N], double (&w)[N]) __attribute__((always_inline)) {
+    constexpr double d = kStep, h = kStep / 2;
+    double r[N];
+    int n[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = fmin(((double)top - (double)x[i]) * per_entry, 960.0 * kTable); // (a mass of 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) n[i] = (int)-r[i]; // (towards zero)
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = lds.table[n[i] & (kTable - 1)];
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = __builtin_amdgcn_fract(r[i]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      double p = __builtin_fma(r[i], -(d * d * d) / 6.0, d * d / 2.0 * (1.0 + h));
+      p = __builtin_fma(p, r[i], -d * (1.0 + h + h * h / 2.0));
+      r[i] = __builtin_fma(p, r[i], 1.0 + h + h * h / 2.0 + h * h * h / 6.0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __builtin_ldexp(r[i] * w[i], (n[i] >> 10) + a.mass_bits) + kRounding;
+  };
   auto units_of = [&](float x) __attribute__((always_inline)) -> u64 {
-    const double y = fmax(((double)x - (double)top) * per_unit, -1200.0); // (nothing from 2^-1075 down)
-    const double t = __builtin_fma(y, (double)kTable, 6755399441055744.0); // 1.5 * 2^52: the rounded n in the low bits
-    const int n = (int)(uint32_t)__builtin_bit_cast(u64, t);
-    const double r = __builtin_fma(t - 6755399441055744.0, -1.0 / kTable, y);
-    constexpr double kLn2 = 0.69314718055994530942;
-    double p = __builtin_fma(r, kLn2 * kLn2 * kLn2 / 6.0, kLn2 * kLn2 / 2.0);
-    p = __builtin_fma(p, r, kLn2);
-    p = __builtin_fma(p, r, 1.0);
-    const double m = __builtin_ldexp(p * lds.table[n & (kTable - 1)], (n >> 10) + a.mass_bits);
-    return __builtin_bit_cast(u64, m + 4503599627370496.0) & 0xfffffffffffffull;
+    double w[1];
+    rounded_masses({x}, w);
+    return __builtin_bit_cast(u64, w[0]) & kMassBits;
   };
   // Steps of the distance to the largest logit, falling as x rises.
   auto step_of = [&](float x, float per_step) __attribute__((always_inline)) -> int {
@@ -394,15 +435,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     const u64 target = (u64)(u * (double)total);
     return target < total ? target : total - 1;
   };
-  auto finish = [&](int token, float x, u64 total) __attribute__((always_inline)) { // (one thread)
+  auto log_of = [&](u64 total) __attribute__((always_inline)) { return log(__builtin_ldexp((double)total, -a.mass_bits)); };
+  auto finish = [&](int token, float x, double log_total) __attribute__((always_inline)) { // (one thread)
     a.tokens[row] = token;
-    if (a.logprobs)
-      a.logprobs[row] = (float)(((double)x - (double)top) / temperature - log(__builtin_ldexp((double)total, -a.mass_bits)));
+    if (a.logprobs) a.logprobs[row] = (float)(((double)x - (double)top) / temperature - log_total);
   };
 
-  auto clear_bins = [&](u64 *bins) __attribute__((always_inline)) {
+  auto clear_bins = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int b = 0; b < kBinsEach; ++b) bins[tid + b * kThreads] = 0;
+    for (int b = 0; b < kBinsEach; ++b) lds.bins[tid + b * kThreads] = 0;
     __syncthreads();
   };
   // f(entry) for this thread's share of the list
@@ -419,7 +460,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
         const float x = static_cast<float>(v[e]);
-        if (x != -INFINITY) f(x, first_of(c, tid) + e);
+        if (x != -INFINITY) f(x, first_of(c, lane) + e);
       }
     });
   };
@@ -431,17 +472,21 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     if (tid == 0) lds.listed = 0;
     __syncthreads();
   };
-  // Up to kRanked listed entries into lds.ranked, in order: four threads (two where
-  // there are more than a quarter of the block) count the entries before one.
-  auto rank_list = [&]() __attribute__((always_inline)) {
-    const int n = lds.listed, share = n <= kThreads / 4 ? 2 : 1, i = tid >> share;
+  // n <= kRanked entries into lds.ranked, in order: four threads (two or one where there
+  // are more than a quarter or half of the block) count the entries before one.
+  auto share_for = [&](int n) __attribute__((always_inline)) {
+    return n <= kThreads / 4 ? 2 : n <= kThreads / 2 ? 1 : 0;
+  };
+  auto rank_entries = [&](const u64 *entries, int n) __attribute__((always_inline)) {
+    const int share = share_for(n), i = tid >> share;
     if (i < n) {
-      const u64 e = lds.list[i];
+      const u64 e = entries[i];
       const int part = tid & ((1 << share) - 1);
       int before = 0;
 #pragma unroll 8
-      for (int j = part; j < n; j += 1 << share) before += lds.list[j] > e ? 1 : 0;
-      before += __builtin_amdgcn_update_dpp(0, before, 0xB1, 0xf, 0xf, true); // (threads of an entry are neighbours)
+      for (int j = part; j < n; j += 1 << share) before += entries[j] > e ? 1 : 0;
+      // (threads of an entry are neighbours)
+      if (share >= 1) before += __builtin_amdgcn_update_dpp(0, before, 0xB1, 0xf, 0xf, true);
       if (share == 2) before += __builtin_amdgcn_update_dpp(0, before, 0x4E, 0xf, 0xf, true);
       if (part == 0) lds.ranked[before] = e;
     }
@@ -463,7 +508,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     for (int level = 0; level < 3; ++level) {
       const int take = level == 2 ? 10 : 11, shift = 32 - bits - take;
       const uint32_t mask = (1u << take) - 1;
-      clear_bins(lds.bins);
+      clear_bins();
       each([&](float x, int index) __attribute__((always_inline)) {
         const uint32_t k = order_key(x);
         if (bits && (k >> (32 - bits)) != r.key) return;
@@ -471,7 +516,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
         if (w) atomicAdd(&lds.bins[mask - ((k >> shift) & mask)], w);
       });
       __syncthreads();
-      const Found f = find_bin(lds, lds.bins, scan_bins(lds, lds.bins), target);
+      const Found f = find_bin(lds, scan_bins<kThreads>(lds), target);
       target -= f.before;
       r.key = r.key << take | (mask - (uint32_t)f.at);
       r.value = f.value;
@@ -480,41 +525,44 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     r.missing = target;
     return r;
   };
-  // Inside segment `f` of the row (the 64 vectors that one wave holds of a chunk): the
-  // index at which the running weight exceeds `target`. Every thread gets it.
-  auto inside_segment = [&](const Found &f, auto &&weight, u64 target) __attribute__((always_inline)) -> int {
-    if (wave == 0) {
-      const int c = f.at / kWaves, t = f.at % kWaves * kWave + lane;
-      const V v = load(c, t);
-      u64 w[kVec], sum = 0;
+  // In the chunk of 64 pieces from `piece` on, which the calling wave takes and before
+  // which the running weight is `before`: f(index, logit) where it exceeds `target`, by one lane.
+  auto inside_chunk = [&](int piece, u64 before, auto &&weight, u64 target, auto &&f) __attribute__((always_inline)) {
+    piece += lane;
+    const V v = load(piece);
+    u64 w[kVec], sum = 0;
+    weight(v, first_in(piece), w);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum += w[e] = weight(static_cast<float>(v[e]), first_of(c, t) + e);
-      u64 at = f.before + wave_scan_u64(sum, lane) - sum;
+    for (int e = 0; e < kVec; ++e) sum += w[e];
+    u64 at = before + wave_scan_u64(sum) - sum;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        if (at <= target && at + w[e] > target) lds.found_at = first_of(c, t) + e; // exactly one
-        at += w[e];
-      }
+    for (int e = 0; e < kVec; ++e) {
+      if (at <= target && at + w[e] > target) f(first_in(piece) + e, static_cast<float>(v[e])); // exactly one
+      at += w[e];
     }
-    __syncthreads();
-    const int index = lds.found_at;
-    __syncthreads();
-    return index;
   };
   // The index of the `ties`-th of the logits equal to x that are in the front.
   auto index_of_tie = [&](float x, u64 ties) __attribute__((always_inline)) -> int {
     auto is_tie = [&](float y, int i) __attribute__((always_inline)) -> u64 { return y == x && in_front(y, i) ? 1 : 0; };
-    clear_bins(lds.bins);
+    clear_bins();
     for_chunks_again([&](int c, const V &v) __attribute__((always_inline)) {
       u64 sum = 0;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum += is_tie(static_cast<float>(v[e]), first_of(c, tid) + e);
+      for (int e = 0; e < kVec; ++e) sum += is_tie(static_cast<float>(v[e]), first_of(c, lane) + e);
       sum = wave_sum_u64(sum);
-      if (lane == 0) lds.bins[c * kWaves + wave] = sum;
+      if (lane == 0) lds.bins[wave * chunks + c] = sum;
     });
     __syncthreads();
-    const Found f = find_bin(lds, lds.bins, scan_bins(lds, lds.bins), ties);
-    return inside_segment(f, is_tie, ties - 1);
+    const Found f = find_bin(lds, scan_bins<kThreads>(lds), ties);
+    if (wave == 0)
+      inside_chunk(f.at * kWave, f.before, [&](const V &v, int first, u64 (&w)[kVec]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) w[e] = is_tie(static_cast<float>(v[e]), first + e);
+      }, ties - 1, [&](int index, float) __attribute__((always_inline)) { lds.found_at = index; });
+    __syncthreads();
+    const int index = lds.found_at;
+    __syncthreads();
+    return index;
   };
   // The front now ends at b.key, of whose logits the first ceil(b.missing / each) are in.
   auto set_cut = [&](const Border &b, u64 each) __attribute__((always_inline)) {
@@ -541,7 +589,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
         continue;
       }
       const u64 mask = (1u << take) - 1;
-      clear_bins(lds.bins);
+      clear_bins();
       const int n = lds.listed;
 #pragma unroll 1
       for (int i = tid; i < n; i += kThreads) {
@@ -551,7 +599,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
         if (w) atomicAdd(&lds.bins[mask - ((e >> (below - take)) & mask)], w);
       }
       __syncthreads();
-      const Found f = find_bin(lds, lds.bins, scan_bins(lds, lds.bins), target);
+      const Found f = find_bin(lds, scan_bins<kThreads>(lds), target);
       target -= f.before;
       prefix = prefix << take | (mask - (u64)f.at);
       below -= take;
@@ -570,12 +618,12 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     if (k <= kThreads) {
       // the step that the k-th largest of the threads' maxima lies in: the logits up to it are at least k
       const float per_step = top > low ? fminf((float)(kBins - 1) / (top - low), 1.0e30f) : 0.f;
-      clear_bins(lds.bins);
+      clear_bins();
       if (mine != -INFINITY) atomicAdd(&lds.bins[step_of(mine, per_step)], (u64)1);
       __syncthreads();
-      const BinScan s = scan_bins(lds, lds.bins);
+      const BinScan<kThreads> s = scan_bins<kThreads>(lds);
       if (s.total >= k) {
-        const Found f = find_bin(lds, lds.bins, s, k);
+        const Found f = find_bin(lds, s, k);
         if (tid == 0) lds.bound = 0xffffffffu;
         start_list();
         if (mine != -INFINITY && step_of(mine, per_step) <= f.at) atomicMin(&lds.bound, order_key(mine));
@@ -585,7 +633,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
 #pragma unroll
           for (int e = 0; e < kVec; ++e) {
             const float x = static_cast<float>(v[e]);
-            if (x >= bound) append(x, first_of(c, at_tid) + e);
+            if (x >= bound) append(x, first_of(c, at_lane) + e);
           }
         });
         __syncthreads();
@@ -595,7 +643,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     }
     if (listed && lds.listed <= kRanked) {
       // everything that is left fits one wave
-      rank_list();
+      rank_entries(lds.list, lds.listed);
       if (wave == 0) {
         const int n = lds.listed < (int)k ? lds.listed : (int)k;
         u64 w[kRankedEach], sum = 0;
@@ -605,7 +653,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
           w[i] = rank < n ? units_of(entry_logit(lds.ranked[rank])) : 0;
           sum += w[i];
         }
-        const u64 upto = wave_scan_u64(sum, lane);
+        const u64 upto = wave_scan_u64(sum);
         const u64 total = wave_sum_u64(sum);
         const u64 target = share_of(total);
         u64 run = upto - sum, kept_sum = 0;
@@ -626,7 +674,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
       }
       __syncthreads();
       // in index order: the threads of an entry sum the kept masses up to its index
-      const int n = lds.listed, share = n <= kThreads / 4 ? 2 : 1, i = tid >> share, part = tid & ((1 << share) - 1);
+      const int n = lds.listed, share = share_for(n), i = tid >> share, part = tid & ((1 << share) - 1);
       const u64 total = lds.found_value, target = drawn_of(total);
       u64 *const units = lds.bins; // (nothing else is in the bins now)
       if (tid < n) units[tid] = units_of(entry_logit(lds.ranked[tid]));
@@ -636,23 +684,23 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
         u64 before = 0;
 #pragma unroll 8
         for (int j = part; j < n; j += 1 << share) before += entry_index(lds.ranked[j]) < index ? units[j] : 0;
-        before += dpp_u64<0xB1>(before);
+        if (share >= 1) before += dpp_u64<0xB1>(before);
         if (share == 2) before += dpp_u64<0x4E>(before);
         if (part == 0 && before <= target && before + units[i] > target)
-          finish(index, entry_logit(lds.ranked[i]), total);
+          finish(index, entry_logit(lds.ranked[i]), log_of(total));
       }
       return;
     }
     if (listed) {
       cut_at(entry_border([](float) __attribute__((always_inline)) -> u64 { return 1; }, k));
     } else { // every logit, where there are more than k of them to count
-      clear_bins(lds.bins);
+      clear_bins();
       u64 count = 0;
       all_again([&](float, int) __attribute__((always_inline)) { ++count; });
       count = wave_sum_u64(count);
       if (lane == 0) lds.bins[wave] = count;
       __syncthreads();
-      const BinScan s = scan_bins(lds, lds.bins);
+      const BinScan<kThreads> s = scan_bins<kThreads>(lds);
       __syncthreads();
       if (s.total > k) set_cut(by_bits(all_again, one_each, k), 1);
     }
@@ -666,32 +714,39 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     // 2048 steps over 2^26 of mass; what is smaller is in the last one and counts as nothing
     constexpr float kPerHalving = (float)(kBins - 1) / 26.0f;
     const float per_step = (float)fmin(kPerHalving * per_unit, 1.0e30);
-    uint32_t *const counts = reinterpret_cast<uint32_t *>(lds.segments);
-    clear_bins(lds.segments);
+#pragma unroll
+    for (int b = 0; b < kBinsEach; ++b) lds.counts[tid + b * kThreads] = 0;
+    const uint32_t beside = kBins + lane; // (what the steps do not hold goes here, a place per lane)
+    __syncthreads();
     for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        const float x = static_cast<float>(v[e]);
-        const int step = step_of(x, per_step);
-        if (step < kBins - 1 && (!cutting || in_front(x, first_of(c, at_tid) + e))) atomicAdd(&counts[step], 1u);
+        float x = static_cast<float>(v[e]);
+        if (cutting && !in_front(x, first_of(c, at_lane) + e)) x = -INFINITY;
+        const uint32_t step = (uint32_t)fminf((top - x) * per_step, (float)(kBins + kWave));
+        atomicAdd(&lds.counts[step < beside ? step : beside], 1u);
       }
     });
     __syncthreads();
     // (2^40 to the largest mass, each taken at the middle of its step)
+    BinScan<kThreads> s;
 #pragma unroll
     for (int i = 0; i < kBinsEach; ++i) {
-      const int b = tid_bin(i);
-      lds.bins[b] = (u64)((float)counts[b] * __builtin_amdgcn_exp2f(40.0f - ((float)b + 0.5f) / kPerHalving));
+      const int b = s.bin(i);
+      s.v[i] = b == kBins - 1 ? 0 : (u64)((float)lds.counts[b] * __builtin_amdgcn_exp2f(40.0f - ((float)b + 0.5f) / kPerHalving));
     }
-    __syncthreads();
-    const BinScan s = scan_bins(lds, lds.bins);
+    s = scan_values(lds, s);
     // Every mass is off by at most a factor 1 +- 0.0044, so a share p by at most 0.0088 p (1 - p).
     const u64 target = share_of(s.total);
     const u64 slack = (u64)((double)s.total * (0.009 * p_setting * (1.0 - p_setting) + 1.0e-5));
-    const Found from = find_bin(lds, lds.bins, s, target > slack ? target - slack : 1);
-    const Found to = find_bin(lds, lds.bins, s, target + slack < s.total ? target + slack : s.total);
-    sure_x = from.at == 0 ? INFINITY : top - ((float)from.at - 0.25f) / per_step;
-    window_x = top - ((float)to.at + 1.25f) / per_step;
+    at_target(s, target > slack ? target - slack : 1,
+              [&](int at, u64, u64) __attribute__((always_inline)) { lds.found_at = at; });
+    at_target(s, target + slack < s.total ? target + slack : s.total,
+              [&](int at, u64, u64) __attribute__((always_inline)) { lds.found_too = at; });
+    __syncthreads();
+    const int from = lds.found_at, to = lds.found_too;
+    sure_x = from == 0 ? INFINITY : top - ((float)from - 0.25f) / per_step;
+    window_x = top - ((float)to + 1.25f) / per_step;
     window = true;
   }
   // Where min-p cuts above the window, nothing in the window stays: the logits that
@@ -702,91 +757,113 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
   auto kept_units = [&](float x, int i) __attribute__((always_inline)) -> u64 {
     return in_front(x, i) && x >= floor_x ? units_of(x) : 0;
   };
+  auto kept_of = [&](const V &v, int first, u64 (&w)[kVec]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e0 = 0; e0 < kVec; e0 += 4) {
+      float x[4];
+      double m[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(v[e0 + e]);
+      rounded_masses(x, m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e0 + e] = in_front(x[e], first + e0 + e) && x[e] >= floor_x ? __builtin_bit_cast(u64, m[e]) & kMassBits : 0;
+    }
+  };
   while (true) {
+    if (tid == 0) lds.num_picked = 0;
     start_list();
-    clear_bins(lds.segments);
-    u64 all = 0; // what top-p is a share of
+    clear_bins();
+    // Whole numbers, at most 2^53 for a thread's logits: 64-bit floats hold their sums exactly.
+    double all = 0.0, kept = 0.0; // what top-p is a share of, and what it surely keeps
     for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
-      u64 kept = 0;
 #pragma unroll
       for (int e0 = 0; e0 < kVec; e0 += 4) { // (four at a time: the masses of eight do not fit the registers)
-        u64 w[4];
-        bool near = false;
+        float x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = units_of(static_cast<float>(v[e0 + e]));
+        for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(v[e0 + e]);
         if (cutting)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = in_front(static_cast<float>(v[e0 + e]), first_of(c, at_tid) + e0 + e) ? w[e] : 0;
+          for (int e = 0; e < 4; ++e) x[e] = in_front(x[e], first_of(c, at_lane) + e0 + e) ? x[e] : -INFINITY;
+        double w[4];
+        rounded_masses(x, w);
+        bool near = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = static_cast<float>(v[e0 + e]);
+          w[e] -= kRounding;
           all += w[e];
-          kept += x > sure_x ? w[e] : 0;
-          near |= x >= window_x && x <= sure_x;
+          // (the upper half alone says nothing: the lower one is then a number below 2^-1022)
+          const u64 bits = __builtin_bit_cast(u64, w[e]);
+          const uint32_t upper = x[e] > sure_x ? (uint32_t)(bits >> 32) : 0u;
+          kept += __builtin_bit_cast(double, (u64)upper << 32 | (uint32_t)bits);
+          near |= x[e] >= window_x && x[e] <= sure_x;
         }
         if (near)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = static_cast<float>(v[e0 + e]);
-            if (x >= window_x && x <= sure_x && w[e]) append(x, first_of(c, at_tid) + e0 + e);
+            if (x[e] >= window_x && x[e] <= sure_x && w[e] > 0.0) append(x[e], first_of(c, at_lane) + e0 + e);
           }
         __builtin_amdgcn_sched_barrier(0);
       }
-      kept = wave_sum_u64(kept);
-      if (lane == 0) lds.segments[c * kWaves + wave] = kept;
     });
+    const u64 wave_kept = wave_sum_u64((u64)kept), wave_all = wave_sum_u64((u64)all);
+    if (lane == 0) lds.wave_kept[wave] = wave_kept, lds.wave_all[wave] = wave_all;
+    __syncthreads();
     if (!window) break;
-    all = wave_sum_u64(all);
-    if (lane == 0) lds.bins[wave] = all;
-    __syncthreads();
-    all = 0;
+    u64 total = 0, above = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) all += lds.bins[w];
-    const u64 above = scan_bins(lds, lds.segments).total;
-    __syncthreads();
-    const u64 target = share_of(all);
+    for (int w = 0; w < kWaves; ++w) total += lds.wave_all[w], above += lds.wave_kept[w];
+    const u64 target = share_of(total);
     const int n = lds.listed;
-    u64 listed_units = 0;
     if (by_floor && above <= target) break;
     if (!by_floor && n <= kListed) {
-      for_listed([&](float x, int) __attribute__((always_inline)) { listed_units += units_of(x); });
-      listed_units = wave_sum_u64(listed_units);
-      if (lane == 0) lds.bins[wave] = listed_units;
+      // the listed ones by their place between the window's ends, in the order of the logits
+      const float from = fminf(sure_x, top), range = from - window_x;
+      const float per_bin = range > 0.f ? fminf((float)(kBins - 1) / range, 1.0e30f) : 0.f;
+      auto bin_of = [&](float x) __attribute__((always_inline)) {
+        return (int)fminf((from - x) * per_bin, (float)(kBins - 1));
+      };
+      for_listed([&](float x, int) __attribute__((always_inline)) { atomicAdd(&lds.bins[bin_of(x)], units_of(x)); });
       __syncthreads();
-      listed_units = 0;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) listed_units += lds.bins[w];
-      __syncthreads();
-    }
-    if (!by_floor && target > above && target <= above + listed_units) {
-      // the border is among the listed ones; those in front of it join their segments
-      if (n <= kRanked) {
-        rank_list();
-        if (wave == 0) {
-          u64 w[kRankedEach], sum = 0;
-#pragma unroll
-          for (int i = 0; i < kRankedEach; ++i) {
-            const int rank = lane * kRankedEach + i;
-            sum += w[i] = rank < n ? units_of(entry_logit(lds.ranked[rank])) : 0;
-          }
-          u64 run = above + wave_scan_u64(sum, lane) - sum;
-#pragma unroll
-          for (int i = 0; i < kRankedEach; ++i) {
-            if (run < target && run + w[i] >= target) lds.found_at = lane * kRankedEach + i; // exactly one
-            run += w[i];
-          }
-        }
+      const BinScan<kThreads> s = scan_bins<kThreads>(lds);
+      if (target > above && target <= above + s.total) {
+        // the border is among the listed ones: in this bin
+        const Found f = find_bin(lds, s, target - above);
+        for_listed([&](float x, int i) __attribute__((always_inline)) {
+          if (bin_of(x) != f.at) return;
+          const int at = atomicAdd(&lds.num_picked, 1);
+          if (at < kRanked) lds.picked[at] = list_entry(x, i);
+        });
         __syncthreads();
-        cut_at(lds.ranked[lds.found_at]);
-      } else {
-        cut_at(entry_border(units_of, target - above));
+        const int picked = lds.num_picked;
+        if (picked == 1) {
+          cut_at(lds.picked[0]);
+        } else if (picked <= kRanked) {
+          rank_entries(lds.picked, picked);
+          if (wave == 0) { // each lane takes ranks one behind the other
+            const int each = (picked + kWave - 1) / kWave, first = lane * each;
+            const int last = first + each < picked ? first + each : picked;
+            u64 sum = 0;
+            for (int i = first; i < last; ++i) sum += units_of(entry_logit(lds.ranked[i]));
+            u64 run = above + f.before + wave_scan_u64(sum) - sum;
+            for (int i = first; i < last; ++i) {
+              const u64 w = units_of(entry_logit(lds.ranked[i]));
+              if (run < target && run + w >= target) lds.found_at = i; // exactly one
+              run += w;
+            }
+          }
+          __syncthreads();
+          cut_at(lds.ranked[lds.found_at]);
+        } else {
+          cut_at(entry_border(units_of, target - above));
+        }
+        // those in front of it join the sums of their waves
+        for_listed([&](float x, int i) __attribute__((always_inline)) {
+          const u64 w = kept_units(x, i);
+          if (w) atomicAdd(&lds.wave_kept[(i + lead) / kVec / kWave / chunks], w);
+        });
+        break;
       }
-      for_listed([&](float x, int i) __attribute__((always_inline)) {
-        const u64 w = kept_units(x, i);
-        if (w) atomicAdd(&lds.segments[(i + lead) / kChunk * kWaves + (i + lead) % kChunk / (kWave * kVec)], w);
-      });
-      break;
     }
     // the hint was off, or its step too full: the exact search, and the pass again without a window
     const Border b = by_bits(all_again, [&](float x, int i) __attribute__((always_inline)) -> u64 {
@@ -798,31 +875,71 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     sure_x = next_below(floor_x);
   }
   __syncthreads();
-  const BinScan s = scan_bins(lds, lds.segments);
-  const u64 target = drawn_of(s.total);
-  const Found f = find_bin(lds, lds.segments, s, target + 1);
-  const int token = inside_segment(f, kept_units, target);
-  if (tid == 0) {
-    const float x = static_cast<float>(logits[token]) + 0.f;
-    finish(token, infinite ? 0.f : x, s.total);
+  // The draw: the wave in whose run of the row the running mass passes the target, its
+  // chunk (every wave sums some), and the logit in it.
+  u64 total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) total += lds.wave_kept[w];
+  const u64 target = drawn_of(total);
+  u64 before = 0;
+  int from = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const u64 upto = before + lds.wave_kept[w];
+    if (upto <= target && from == w) before = upto, from = w + 1;
   }
+  const int first_chunk = from * chunks; // (from < kWaves: the target is below the total)
+  if (wave == kWaves - 1) { // (the wave that has the fewest of the chunks below)
+    const double log_total = log_of(total);
+    if (lane == 0) lds.log_total = log_total;
+  }
+#pragma unroll 1
+  for (int c = wave; c < chunks; c += kWaves) {
+    const int piece = (first_chunk + c) * kWave + lane;
+    const V v = load(piece);
+    u64 w[kVec], sum = 0;
+    kept_of(v, first_in(piece), w);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum += w[e];
+    sum = wave_sum_u64(sum);
+    if (lane == 0) lds.list[c] = sum; // (the list is read no more)
+  }
+  __syncthreads();
+  int c = 0;
+#pragma unroll 8
+  for (int i = 0; i < chunks - 1; ++i) {
+    const u64 upto = before + lds.list[i];
+    if (upto <= target && c == i) before = upto, c = i + 1;
+  }
+  if (wave == c % kWaves)
+    inside_chunk((first_chunk + c) * kWave, before, kept_of, target, [&](int index, float x)
+                     __attribute__((always_inline)) { finish(index, x, lds.log_total); });
 }
 
-// Logits a row may have: its segments have to fit the bins.
+// Logits a row may have: its chunks have to fit the bins, and the list.
 constexpr int64_t kMaxVocab = 500000;
-static_assert(kMaxVocab + 8 <= (int64_t)kBins / kWaves * kThreads * 4, "a bin per segment");
+// A block of 1024 threads per row while every row gets a CU of its own.
+constexpr int64_t kRowsAtOnce = 256;
+static_assert(kMaxVocab + 8 <= (int64_t)kBins * kWave * 4 - kMostWaves * kWave * 4, "a bin per chunk");
 
-template <typename T>
-int launch_sample(const SampleArgs &a, int64_t rows, hipStream_t stream) {
-  constexpr int kChunk = kThreads * Io<T>::kVec;
+template <typename T, int kThreads>
+int launch_sample_threads(const SampleArgs &a, int64_t rows, hipStream_t stream) {
+  constexpr int kChunk = kThreads * Io<T>::kVec, kMostInLds = most_in_lds(kThreads);
   const int chunks = (a.vocab + Io<T>::kVec - 1 + kChunk - 1) / kChunk;
   const int in_lds = chunks <= kInRegisters ? 0 : chunks - kInRegisters < kMostInLds ? chunks - kInRegisters : kMostInLds;
   const unsigned bytes = (unsigned)(sizeof(SampleLds) + (size_t)in_lds * kThreads * 16);
   constexpr unsigned kMostBytes = (unsigned)(sizeof(SampleLds) + (size_t)kMostInLds * kThreads * 16);
-  const int s = raise_lds_limit(reinterpret_cast<const void *>(sample_kernel<T>), kMostBytes, "oslo_sample");
+  static_assert(kMostBytes * (1024 / kThreads) <= 160 * 1024, "of a CU");
+  const int s = raise_lds_limit(reinterpret_cast<const void *>(sample_kernel<T, kThreads>), kMostBytes, "oslo_sample");
   if (s != OSLO_OK) return s;
-  sample_kernel<T><<<dim3((unsigned)rows), dim3(kThreads), bytes, stream>>>(a);
+  sample_kernel<T, kThreads><<<dim3((unsigned)rows), dim3(kThreads), bytes, stream>>>(a);
   return check_launch("sample");
+}
+
+template <typename T>
+int launch_sample(const SampleArgs &a, int64_t rows, hipStream_t stream) {
+  if (rows > kRowsAtOnce) return launch_sample_threads<T, 512>(a, rows, stream);
+  return launch_sample_threads<T, 1024>(a, rows, stream);
 }
 
 } // namespace
@@ -854,7 +971,7 @@ extern "C" int oslo_sample(int64_t *tokens, float *logprobs, const void *logits,
   a.vocab = (int)vocab;
   int log2_vocab = 0;
   while (((int64_t)1 << log2_vocab) < vocab) ++log2_vocab;
-  a.mass_bits = 62 - log2_vocab < 51 ? 62 - log2_vocab : 51;
+  a.mass_bits = 61 - log2_vocab < 49 ? 61 - log2_vocab : 49; // (a thread's sum is at most 2^53)
   hipStream_t st = static_cast<hipStream_t>(stream);
   OSLO_DISPATCH_DTYPE(dtype, return launch_sample<T>(a, rows, st));
   return OSLO_OK;

@@ -178,3 +178,22 @@ def test_refused_calls():
         with pytest.raises(RuntimeError):
             FusedSampling.apply(*args)
     assert FusedSampling.apply(logits[:0], u[:0])[0].shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 17, 1000, 5001, 50257])
+def test_many_rows_draw_as_few_do(vocab, dtype):
+    """Numbers of rows on both sides of the change of block size: the same tokens, the same bits."""
+    rows = 260
+    g = torch.Generator().manual_seed(vocab)
+    logits = (torch.randn((rows, vocab), generator=g) * 3).to(dtype).to(DEV)
+    logits[5], logits[6] = 1.0, float("-inf")
+    logits[7, vocab // 2:] = float("inf")
+    u = torch.rand(rows, generator=g).to(DEV)
+    settings = [dict(), dict(top_k=50), dict(top_k=400, top_p=0.9), dict(top_k=3000, top_p=0.95, temperature=0.7),
+                dict(top_p=0.92), dict(top_p=0.5, min_p=0.01), dict(min_p=0.1, temperature=1.5), dict(temperature=0.0)]
+    for kw in settings:
+        many = FusedSampling.apply(logits, u, **kw)
+        few = [FusedSampling.apply(logits[i:i + 130], u[i:i + 130], **kw) for i in (0, 130)]
+        assert torch.equal(many[0], torch.cat([t for t, _ in few])), kw
+        assert torch.equal(many[1], torch.cat([p for _, p in few])), kw
