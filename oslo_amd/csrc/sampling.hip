@@ -287,6 +287,9 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
   for (int c = 0; c < kInRegisters; ++c) clean(held[c], piece_of(c, lane));
 #pragma unroll 1
   for (int i = tid; i < kTable; i += kThreads) lds.table[i] = table_entry(i);
+#pragma unroll
+  for (int b = 0; b < kBinsEach; ++b) lds.bins[tid + b * kThreads] = 0;
+  if (tid == 0) lds.listed = 0;
   // f(chunk, vector) for every vector of this thread. The empty statement "changes"
   // the vector: without it the compiler works out ahead, for all chunks at once, what
   // several passes have in common (conversions, whole masses, indices), and spills it.
@@ -477,7 +480,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
   auto share_for = [&](int n) __attribute__((always_inline)) {
     return n <= kThreads / 4 ? 2 : n <= kThreads / 2 ? 1 : 0;
   };
-  auto rank_entries = [&](const u64 *entries, int n) __attribute__((always_inline)) {
+  // f(rank, entry) for each.
+  auto rank_entries = [&](const u64 *entries, int n, auto &&f) __attribute__((always_inline)) {
     const int share = share_for(n), i = tid >> share;
     if (i < n) {
       const u64 e = entries[i];
@@ -488,7 +492,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
       // (threads of an entry are neighbours)
       if (share >= 1) before += __builtin_amdgcn_update_dpp(0, before, 0xB1, 0xf, 0xf, true);
       if (share == 2) before += __builtin_amdgcn_update_dpp(0, before, 0x4E, 0xf, 0xf, true);
-      if (part == 0) lds.ranked[before] = e;
+      if (part == 0) {
+        lds.ranked[before] = e;
+        f(before, e);
+      }
     }
     __syncthreads();
   };
@@ -617,18 +624,16 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     bool listed = false;
     if (k <= kThreads) {
       // the step that the k-th largest of the threads' maxima lies in: the logits up to it are at least k
+      // (the bins and the list have been cleared with the row's load)
       const float per_step = top > low ? fminf((float)(kBins - 1) / (top - low), 1.0e30f) : 0.f;
-      clear_bins();
       if (mine != -INFINITY) atomicAdd(&lds.bins[step_of(mine, per_step)], (u64)1);
       __syncthreads();
       const BinScan<kThreads> s = scan_bins<kThreads>(lds);
       if (s.total >= k) {
         const Found f = find_bin(lds, s, k);
-        if (tid == 0) lds.bound = 0xffffffffu;
-        start_list();
-        if (mine != -INFINITY && step_of(mine, per_step) <= f.at) atomicMin(&lds.bound, order_key(mine));
-        __syncthreads();
-        const float bound = key_value(lds.bound); // the smallest of those maxima, of which there are at least k
+        // at or below the smallest number of that step: of the margin, a hundredth is for the product's rounding,
+        // the next number below for the difference's
+        const float bound = per_step > 0.f ? next_below(top - ((float)f.at + 1.01f) / per_step) : low;
         for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
 #pragma unroll
           for (int e = 0; e < kVec; ++e) {
@@ -643,14 +648,17 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     }
     if (listed && lds.listed <= kRanked) {
       // everything that is left fits one wave
-      rank_entries(lds.list, lds.listed);
+      u64 *const units = lds.bins; // (nothing else is in the bins now)
+      rank_entries(lds.list, lds.listed, [&](int rank, u64 e) __attribute__((always_inline)) {
+        units[rank] = units_of(entry_logit(e));
+      });
       if (wave == 0) {
         const int n = lds.listed < (int)k ? lds.listed : (int)k;
         u64 w[kRankedEach], sum = 0;
 #pragma unroll
         for (int i = 0; i < kRankedEach; ++i) {
           const int rank = lane * kRankedEach + i;
-          w[i] = rank < n ? units_of(entry_logit(lds.ranked[rank])) : 0;
+          w[i] = rank < n ? units[rank] : 0;
           sum += w[i];
         }
         const u64 upto = wave_scan_u64(sum);
@@ -676,19 +684,21 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
       // in index order: the threads of an entry sum the kept masses up to its index
       const int n = lds.listed, share = share_for(n), i = tid >> share, part = tid & ((1 << share) - 1);
       const u64 total = lds.found_value, target = drawn_of(total);
-      u64 *const units = lds.bins; // (nothing else is in the bins now)
-      if (tid < n) units[tid] = units_of(entry_logit(lds.ranked[tid]));
-      __syncthreads();
+      u64 before = 0;
       if (i < n) {
         const int index = entry_index(lds.ranked[i]);
-        u64 before = 0;
 #pragma unroll 8
         for (int j = part; j < n; j += 1 << share) before += entry_index(lds.ranked[j]) < index ? units[j] : 0;
         if (share >= 1) before += dpp_u64<0xB1>(before);
         if (share == 2) before += dpp_u64<0x4E>(before);
-        if (part == 0 && before <= target && before + units[i] > target)
-          finish(index, entry_logit(lds.ranked[i]), log_of(total));
       }
+      if (wave == kWaves - 1) { // (hardly ever one of those that counted)
+        const double log_total = log_of(total);
+        if (lane == 0) lds.log_total = log_total;
+      }
+      __syncthreads();
+      if (i < n && part == 0 && before <= target && before + units[i] > target)
+        finish(entry_index(lds.ranked[i]), entry_logit(lds.ranked[i]), lds.log_total);
       return;
     }
     if (listed) {
@@ -839,7 +849,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
         if (picked == 1) {
           cut_at(lds.picked[0]);
         } else if (picked <= kRanked) {
-          rank_entries(lds.picked, picked);
+          rank_entries(lds.picked, picked, [](int, u64) __attribute__((always_inline)) {});
           if (wave == 0) { // each lane takes ranks one behind the other
             const int each = (picked + kWave - 1) / kWave, first = lane * each;
             const int last = first + each < picked ? first + each : picked;
