@@ -471,6 +471,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     const int at = atomicAdd(&lds.listed, 1);
     if (at < kListed) lds.list[at] = list_entry(x, index);
   };
+  auto pick = [&](float x, int index) __attribute__((always_inline)) {
+    const int at = atomicAdd(&lds.num_picked, 1);
+    if (at < kRanked) lds.picked[at] = list_entry(x, index);
+  };
   auto start_list = [&]() __attribute__((always_inline)) {
     if (tid == 0) lds.listed = 0;
     __syncthreads();
@@ -622,6 +626,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
   if (k_setting > 1.0 && k_setting < (double)vocab) {
     const u64 k = (u64)k_setting;
     bool listed = false;
+    float bound = -INFINITY;
     if (k <= kThreads) {
       // the step that the k-th largest of the threads' maxima lies in: the logits up to it are at least k
       // (the bins and the list have been cleared with the row's load)
@@ -633,7 +638,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
         const Found f = find_bin(lds, s, k);
         // at or below the smallest number of that step: of the margin, a hundredth is for the product's rounding,
         // the next number below for the difference's
-        const float bound = per_step > 0.f ? next_below(top - ((float)f.at + 1.01f) / per_step) : low;
+        bound = per_step > 0.f ? next_below(top - ((float)f.at + 1.01f) / per_step) : low;
         for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
 #pragma unroll
           for (int e = 0; e < kVec; ++e) {
@@ -646,14 +651,31 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
       }
       __syncthreads();
     }
-    if (listed && lds.listed <= kRanked) {
+    const u64 *entries = lds.list;
+    int num_entries = lds.listed;
+    if (listed && num_entries > kRanked && k <= kRanked) {
+      // too many to rank: those in finer steps between the bound and the largest, up to the step of the k-th
+      const float range = top - bound;
+      const float per_bin = range > 0.f ? fminf((float)(kBins - 1) / range, 1.0e30f) : 0.f;
+      if (tid == 0) lds.num_picked = 0;
+      clear_bins();
+      for_listed([&](float x, int) __attribute__((always_inline)) { atomicAdd(&lds.bins[step_of(x, per_bin)], (u64)1); });
+      __syncthreads();
+      const Found f = find_bin(lds, scan_bins<kThreads>(lds), k);
+      for_listed([&](float x, int i) __attribute__((always_inline)) {
+        if (step_of(x, per_bin) <= f.at) pick(x, i);
+      });
+      __syncthreads();
+      if (lds.num_picked <= kRanked) entries = lds.picked, num_entries = lds.num_picked;
+    }
+    if (listed && num_entries <= kRanked) {
       // everything that is left fits one wave
       u64 *const units = lds.bins; // (nothing else is in the bins now)
-      rank_entries(lds.list, lds.listed, [&](int rank, u64 e) __attribute__((always_inline)) {
+      rank_entries(entries, num_entries, [&](int rank, u64 e) __attribute__((always_inline)) {
         units[rank] = units_of(entry_logit(e));
       });
       if (wave == 0) {
-        const int n = lds.listed < (int)k ? lds.listed : (int)k;
+        const int n = num_entries < (int)k ? num_entries : (int)k;
         u64 w[kRankedEach], sum = 0;
 #pragma unroll
         for (int i = 0; i < kRankedEach; ++i) {
@@ -840,9 +862,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
         // the border is among the listed ones: in this bin
         const Found f = find_bin(lds, s, target - above);
         for_listed([&](float x, int i) __attribute__((always_inline)) {
-          if (bin_of(x) != f.at) return;
-          const int at = atomicAdd(&lds.num_picked, 1);
-          if (at < kRanked) lds.picked[at] = list_entry(x, i);
+          if (bin_of(x) == f.at) pick(x, i);
         });
         __syncthreads();
         const int picked = lds.num_picked;
