@@ -34,7 +34,8 @@
 // positions), and nothing but the lengths in device memory decides, so a captured
 // step follows them when it is replayed. A sequence of one chunk is finished there; the
 // chunks of longer ones leave partial results (maximum, sum, fp32 accumulator) that
-// a second kernel joins in order.
+// a second kernel joins in order. Where the cache holds short sequences only, a block
+// takes a whole one instead (MEET): the second launch cost more than the meeting.
 
 #include <algorithm>
 
@@ -238,7 +239,8 @@ __device__ __forceinline__ int list_chunks(const PagedDecodeArgs &a, int *first,
 // instead of 96 at 131071 positions; six at 64: 81 instead of 56 at 8 x 16000 positions.)
 constexpr int blocks_per_cu(int D) { return D == 256 ? 2 : D == 128 ? 3 : 4; }
 
-template <typename T, int D, bool E4M3>
+// MEET: a block per sequence and head slot, whose waves share its tiles and meet in LDS.
+template <typename T, int D, bool E4M3, bool MEET>
 __global__ __launch_bounds__(kBlockThreads, blocks_per_cu(D)) void attention_paged_decode_kernel(const PagedDecodeArgs a) {
   using Op = Mfma16<T>;
   using Frag = typename Op::Frag;
@@ -256,32 +258,39 @@ __global__ __launch_bounds__(kBlockThreads, blocks_per_cu(D)) void attention_pag
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int col = lane & 15, g = lane >> 4;
 
-  const int chunk_keys = list_chunks(a, first_chunk, &turn[0][0][0]);
-  if (a.plan != nullptr && blockIdx.x == 0) {
+  const int chunk_keys = MEET ? 0 : list_chunks(a, first_chunk, &turn[0][0][0]);
+  if (!MEET && a.plan != nullptr && blockIdx.x == 0) {
     for (int i = threadIdx.x; i <= a.map.sequences; i += kBlockThreads) a.plan[i] = first_chunk[i];
     if (threadIdx.x == 0) a.plan[a.map.sequences + 1] = chunk_keys;
   }
   const int slots = a.map.kv_heads * a.column_groups;
-  const unsigned items = (unsigned)first_chunk[a.map.sequences] * (unsigned)slots;
+  const unsigned items = (unsigned)(MEET ? a.map.sequences : first_chunk[a.map.sequences]) * (unsigned)slots;
 
 #pragma unroll 1
-  for (unsigned item = blockIdx.x + (unsigned)wave * gridDim.x; item < items; item += gridDim.x * kWavesPerBlock) {
+  for (unsigned item = blockIdx.x + (MEET ? 0u : (unsigned)wave * gridDim.x); item < items;
+       item += gridDim.x * (MEET ? 1 : kWavesPerBlock)) {
   const int head_slot = (int)(item % (unsigned)slots);
   const int chunk_index = (int)(item / (unsigned)slots);
-  int seq = 0; // the last sequence whose first chunk is not behind this one
-  for (int step = 1 << (31 - __builtin_clz(a.map.sequences)); step > 0; step >>= 1)
-    if (seq + step < a.map.sequences && first_chunk[seq + step] <= chunk_index) seq += step;
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  const int chunk = __builtin_amdgcn_readfirstlane(chunk_index - first_chunk[seq]);
-  const bool alone = __builtin_amdgcn_readfirstlane(first_chunk[seq + 1] - first_chunk[seq]) == 1;
+  int seq = MEET ? chunk_index : 0, chunk = 0;
+  bool alone = false;
+  if constexpr (!MEET) { // the last sequence whose first chunk is not behind this one
+    for (int step = 1 << (31 - __builtin_clz(a.map.sequences)); step > 0; step >>= 1)
+      if (seq + step < a.map.sequences && first_chunk[seq + step] <= chunk_index) seq += step;
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    chunk = __builtin_amdgcn_readfirstlane(chunk_index - first_chunk[seq]);
+    alone = __builtin_amdgcn_readfirstlane(first_chunk[seq + 1] - first_chunk[seq]) == 1;
+  }
   const int kv_head = head_slot / a.column_groups;
   const int column0 = (head_slot % a.column_groups) * kColumns; // the first head of the group this block takes
   const int columns = a.group - column0 < kColumns ? a.group - column0 : kColumns;
   const int head0 = kv_head * a.group + column0;
 
   const Visible vis = visible_of(a, seq);
-  const int tile0 = tiles_begin(vis) + chunk * chunk_keys;
-  const int key_end = vis.last + 1 - tile0 < chunk_keys ? vis.last + 1 : tile0 + chunk_keys;
+  const int begin = tiles_begin(vis);
+  const int share = MEET ? ((vis.last + kTileKeys - begin) / kTileKeys + kWavesPerBlock - 1) / kWavesPerBlock * kTileKeys
+                         : chunk_keys;
+  const int tile0 = begin + (MEET ? wave : chunk) * share;
+  const int key_end = vis.last + 1 - tile0 < share ? vis.last + 1 : tile0 + share;
   if (vis.last < vis.first) { // nothing to see
     for (int i = lane; i < columns * D; i += kWave)
       static_cast<T *>(a.out)[((int64_t)seq * a.heads + head0) * D + i] = static_cast<T>(0.f);
@@ -512,8 +521,12 @@ __global__ __launch_bounds__(kBlockThreads, blocks_per_cu(D)) void attention_pag
   float(*const mine)[D + 4] = turn[wave];
 #pragma unroll 1
   for (int c0 = 0; c0 < columns; c0 += kTurned) {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); // (the rows before have been read)
-    __builtin_amdgcn_wave_barrier();
+    if constexpr (MEET) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); // (the rows before have been read)
+      __builtin_amdgcn_wave_barrier();
+    }
     if (col >= c0 && col < c0 + kTurned) {
 #pragma unroll
       for (int i = 0; i < kBlocksD; ++i)
@@ -526,7 +539,30 @@ __global__ __launch_bounds__(kBlockThreads, blocks_per_cu(D)) void attention_pag
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     const int rows_here = columns - c0 < kTurned ? columns - c0 : kTurned;
-    if (alone) {
+    if constexpr (MEET) {
+      __syncthreads();
+      // the waves' sums in order, relative to their common maximum (a wave without keys has -inf, and zeros)
+      for (int i = threadIdx.x; i < rows_here * (D / 4); i += kBlockThreads) {
+        const int c = i / (D / 4), d = 4 * (i % (D / 4));
+        float top = turn[0][c][D], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWavesPerBlock; ++w) top = fmaxf(top, turn[w][c][D]);
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWavesPerBlock; ++w) {
+          const float alpha = turn[w][c][D] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(turn[w][c][D] - top);
+          const f32x4 v = *reinterpret_cast<const f32x4 *>(&turn[w][c][d]);
+          sum = __builtin_fmaf(turn[w][c][D + 1], alpha, sum);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], alpha, x[e]);
+        }
+        typename VecOf<T, 4>::type y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(x[e] / sum);
+        *reinterpret_cast<typename VecOf<T, 4>::type *>(
+            static_cast<T *>(a.out) + ((int64_t)seq * a.heads + head0 + c0 + c) * D + d) = y;
+      }
+    } else if (alone) {
       constexpr int kRowLanes = D / 8; // lanes that store a row, eight features each
       for (int c = lane / kRowLanes; c < rows_here; c += kWave / kRowLanes) {
         const float inverse = 1.0f / mine[c][D + 1];
@@ -595,6 +631,13 @@ __global__ __launch_bounds__(kBlockThreads) void attention_paged_join_kernel(con
   }
 }
 
+// Where a sequence can have no more than so many tiles, a block takes it: its waves meet
+// in LDS, and one launch is all. In us, against chunks and a join, with the blocks there are:
+//   64 features x 12 heads:  1 x 300 positions 4.4 (7.4), 4 x 300 5.7 (8.0), 32 x 1024 15.2 (16.3), 400 x 1024 111 (122);
+//   128 x 8, 32 query heads: 4 x 512 7.8 (8.9), 4 x 1024 14.2 (10.5), 32 x 1024 19.6 (22.5), 32 x 2048 33 (31);
+//   256 x 16:                4 x 256 7.7 (9.8), 1 x 512 13.7 (8.8), 16 x 512 17.7 (19.2), 32 x 2048 116 (95).
+inline int64_t meet_tiles(int64_t blocks, int64_t head_dim) { return blocks >= 256 ? 32 : head_dim == 256 ? 8 : 16; }
+
 // The grid: as many blocks as fit the card's 256 CUs at a time, or fewer where the
 // sequences cannot have so many chunks. What the workspace has to hold follows from
 // it: the chunk size makes at most full_chunks() chunks of all keys and heads, and
@@ -602,6 +645,7 @@ __global__ __launch_bounds__(kBlockThreads) void attention_paged_join_kernel(con
 struct DecodeGrid {
   int64_t blocks, chunks; // chunks: at most, of one head slot
   bool join;              // some sequence may have more than one
+  bool meet;              // a block takes a whole sequence
 };
 inline DecodeGrid decode_grid(int64_t sequences, int64_t kv_heads, int64_t column_groups, int64_t head_dim,
                               int64_t max_length, int64_t window) {
@@ -610,6 +654,13 @@ inline DecodeGrid decode_grid(int64_t sequences, int64_t kv_heads, int64_t colum
   const int64_t per_sequence = std::max<int64_t>(1, (span + kMinChunk - 1) / kMinChunk);
   const int64_t slots = kv_heads * column_groups;
   DecodeGrid g;
+  g.meet = per_sequence > 1 && per_sequence <= meet_tiles(sequences * slots, head_dim);
+  if (g.meet) {
+    g.blocks = sequences * slots;
+    g.chunks = 0;
+    g.join = false;
+    return g;
+  }
   // (few chunks: a block for each, so that they spread over the CUs)
   g.blocks = std::min<int64_t>(256 * blocks_per_cu((int)head_dim), sequences * per_sequence * slots);
   g.chunks = std::min(sequences * per_sequence,
@@ -635,8 +686,11 @@ int launch_paged_decode(PagedDecodeArgs a, int64_t max_length, hipStream_t strea
     part.full_chunks = (double)full_chunks(kWavesPerBlock * grid.blocks, n * slots) / (double)slots;
     part.plan = grid.join ? reinterpret_cast<int *>(a.partial) : nullptr;
     part.partial = grid.join ? a.partial + plan_ints(n) : nullptr;
-    auto *kernel = a.key_scales ? attention_paged_decode_kernel<T, D, true> : attention_paged_decode_kernel<T, D, false>;
-    const unsigned list_bytes = (unsigned)((n + 1) * sizeof(int));
+    auto *kernel = grid.meet ? (a.key_scales ? attention_paged_decode_kernel<T, D, true, true>
+                                             : attention_paged_decode_kernel<T, D, false, true>)
+                             : (a.key_scales ? attention_paged_decode_kernel<T, D, true, false>
+                                             : attention_paged_decode_kernel<T, D, false, false>);
+    const unsigned list_bytes = grid.meet ? 0u : (unsigned)((n + 1) * sizeof(int));
     kernel<<<dim3((unsigned)grid.blocks), dim3(kBlockThreads), list_bytes, stream>>>(part);
     int s = check_launch("attention_paged_decode");
     if (s != OSLO_OK) return s;

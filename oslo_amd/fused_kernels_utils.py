@@ -36,7 +36,11 @@ def _needs_grad(*tensors):
     """False when autograd would record nothing: the operators then call the
     kernels directly and skip the autograd.Function machinery (a decoding step
     is bound by such per-call overheads, not by its kernels)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def get_custom_kernels():
@@ -682,20 +686,22 @@ class FusedPrefillAttention(object):
         return get_custom_kernels().attention_prefill_forward(query, key, value, scale, pad, window or 0)
 
 
-def _check_captured_leaves(*tensors):
+def _check_captured_leaves(out):
     """A leaf's gradient is added up on the stream of the first graph that holds
     it. Captured into a HIP graph while an eager graph of that leaf lives, that
     addition would leave the capture and end the process: it is refused instead.
-    The caller keeps what is returned until its own graph holds the leaves."""
-    capturing = all(t.is_cuda for t in tensors) and torch.cuda.is_current_stream_capturing()
-    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in tensors if t.is_leaf and t.requires_grad]
-    for node in nodes:
+    ``out``: a recorded result, whose graph holds the leaves by now."""
+    capturing = None
+    for node, _ in out.grad_fn.next_functions:
+        if getattr(node, "variable", None) is None:  # (not a leaf)
+            continue
+        if capturing is None:
+            capturing = torch.cuda.is_current_stream_capturing()
         if not capturing:
             node.metadata["oslo_amd.eager"] = True  # gone with the last eager graph of the leaf
         elif "oslo_amd.eager" in node.metadata:
             raise RuntimeError("captured while an eager graph of the same leaf lives: drop that graph's outputs "
                                "(or use a detached copy) first")
-    return nodes
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -750,8 +756,9 @@ class FusedPackedAttention(object):
         """``window``: query i sees the keys i - window < s <= i of its sequence."""
         scale = 1.0 if scale is None else scale
         if _needs_grad(query, key, value):
-            leaves = _check_captured_leaves(query, key, value)  # noqa: F841
-            return _PackedAttention.apply(query, key, value, packed, scale, window or 0)
+            out = _PackedAttention.apply(query, key, value, packed, scale, window or 0)
+            _check_captured_leaves(out)
+            return out
         return get_custom_kernels().attention_packed_forward(query, key, value, packed, scale, window or 0)
 
 

@@ -9,6 +9,7 @@ implementation: a CPU tensor is rejected with ``RuntimeError``.
 """
 
 import ctypes
+import functools
 
 import torch
 
@@ -765,17 +766,27 @@ def _packed_args(query, key, value, packed):
     return code
 
 
+@functools.lru_cache(maxsize=256)
+def _strides_of(*flat):
+    return _Strides[len(flat)](*flat)
+
+
 def _token_strides(*tensors):
     flat = []
     for t in tensors:
         st, sh, _ = t.stride()
         flat += (sh, st)
-    return _Strides[len(flat)](*flat)
+    return _strides_of(*flat)
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_workspace_floats(*sizes):
+    return _lib.load().oslo_attention_paged_decode_workspace_bytes(*sizes) // 4
 
 
 def _packed_empty(tokens, heads, d, packed, like):
     """An uninitialised [tokens, heads, D] whose rows behind the last sequence are zeros."""
-    out = torch.empty((tokens, heads, d), dtype=like.dtype, device=like.device)
+    out = like.new_empty((tokens, heads, d))
     if packed.total < tokens:
         out[packed.total:].zero_()
     return out
@@ -916,13 +927,13 @@ def attention_paged_decode_forward(query, cache, lengths, scale, window=0):
         q = q.clone(memory_format=torch.contiguous_format)
         qb, qh, _ = q.stride()
     lib = _lib.load()
-    nbytes = lib.oslo_attention_paged_decode_workspace_bytes(b, h, hkv, d, counts[1] * page, window)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
-    out = torch.empty((b, h, d), dtype=q.dtype, device=q.device)
+    floats = _decode_workspace_floats(b, h, hkv, d, counts[1] * page, window)
+    ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    out = q.new_empty((b, h, d))
     with _on_device(q):
         _lib.check(lib.oslo_attention_paged_decode_fwd(
             out.data_ptr(), q.data_ptr(), *pointers, cache.table.data_ptr(), lengths.data_ptr(), _ptr(ws), scale,
-            *counts, h, hkv, page, d, window, _Strides[2](qb, qh), code, _stream(q)))
+            *counts, h, hkv, page, d, window, _strides_of(qb, qh), code, _stream(q)))
     return out
 
 
@@ -955,8 +966,8 @@ def sample_forward(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=
     min_p, min_p_all = _row_setting(min_p, "min_p", torch.float32, rows, logits)
     x = logits if logits.stride(1) == 1 else logits.contiguous()
     uniforms = uniforms.contiguous()
-    tokens = torch.empty((rows,), dtype=torch.int64, device=x.device)
-    logprobs = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    tokens = x.new_empty((rows,), dtype=torch.int64)
+    logprobs = uniforms.new_empty((rows,))
     with _on_device(x):
         _lib.check(_lib.load().oslo_sample(
             tokens.data_ptr(), logprobs.data_ptr(), x.data_ptr(), uniforms.data_ptr(), _ptr(temperature),
