@@ -64,12 +64,14 @@ class _NoSwitch(object):
 
 
 _NO_SWITCH = _NoSwitch()
+# (a device tensor exists, so there is nothing left to initialise)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _on_device(t):
     """Context that makes t's device current for the launch; nothing to do (and
     nothing to pay) when it already is."""
-    if t.device.index == torch.cuda.current_device():
+    if t.device.index == _current_device():
         return _NO_SWITCH
     return torch.cuda.device(t.device)
 
