@@ -305,11 +305,20 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
         __builtin_amdgcn_sched_barrier(0);
       }
     at_lane = lane;
+    // (what is read again is on its way while the chunk before it is worked on)
+    V ahead{};
+    if (chunks > kInRegisters + kMostInLds) ahead = load_raw(piece_of(kInRegisters + kMostInLds, lane));
 #pragma unroll 1
     for (int c = kInRegisters; c < chunks; ++c) {
       V v;
-      if (c < kInRegisters + kMostInLds) v = lds_held[(c - kInRegisters) * kThreads + tid];
-      else v = load(piece_of(c, lane));
+      if (c < kInRegisters + kMostInLds) {
+        v = lds_held[(c - kInRegisters) * kThreads + tid];
+      } else {
+        v = ahead;
+        ahead = load_raw(piece_of(c + 1, lane));
+        clean(v, piece_of(c, lane));
+        if (infinite) only_infinite(v);
+      }
       f(c, v);
     }
   };
