@@ -17,23 +17,30 @@
 // times finer than a 32-bit sum). Sums of whole numbers are exact in any order:
 // histograms may use atomics and every run gives the same token.
 //
-// One block of 1024 threads takes a row and holds it in registers and LDS (53248
-// logits of 32 bits; what exceeds them is read again), so memory is read once. What costs the
-// time then is arithmetic, thirty instructions a logit, and barriers:
+// One block takes a row, 1024 threads and a CU for itself up to 256 rows; beyond that
+// 512, two to a CU, one waiting for memory or at a barrier while the other computes
+// (1000 rows of 50257 fp32 logits with top-p: 127 against 155 us). It holds the row in
+// registers and LDS (53248 logits of 32 bits, or 20480, twice that in 16 bits; what exceeds them
+// is read again, ahead of its use), each wave a run of it. Such a row is read in 5 to 8 us; what
+// costs the time then is arithmetic, one operation in 64 bits after another, and
+// barriers (one row of 1024 threads, thousands of cycles: reading 10, the count below 12, its
+// border 4, the exact pass 30, the border in the window 5 to 7, the draw 11):
 //  - top-k goes first: a histogram of the threads' own maxima gives a bound that
 //    at least k logits reach and few exceed. They go into a list in LDS, which is all
 //    the rest looks at; up to 512 of them are ranked by counting, without a sort.
 //  - top-p over a whole row: the logits are counted over 2048 steps of the distance to
 //    the largest one. Masses inside a step differ by 0.9 %, so the counts place the border
 //    of a share p to 0.9 % p (1 - p) of the mass, a step or a few. The one exact pass
-//    then sums all masses, sums those in front of that window by segments of the row, and
+//    then sums all masses, sums those in front of that window by waves, and
 //    lists the logits in the window; the exact sums say whether the border really is among the listed ones
-//    (else an exact search finds it: the hint never decides). The listed ones are
-//    ranked.
-//  - the draw finds the segment in which the running mass passes its target, and
-//    looks inside it.
+//    (else an exact search finds it: the hint never decides). The listed ones' masses are summed over
+//    finer steps, and the few in the step of the border are ranked (all of them ranked
+//    by counting took 34 thousand cycles, this 5 to 7).
+//  - the draw finds the wave in whose run the running mass passes its target, its
+//    chunk, which all waves sum together, and looks inside that.
 // Windows too full for the list (equal logits by the thousand) are searched by
-// histograms over the bits of the logits.
+// histograms over the bits of the logits. Measured, us a call: one row of 50257 fp32 logits, top-k 50 and
+// top-p, 12.6; 256 rows in bf16, settings of their own, 39; 1000 rows in fp32, top-p 0.92, 127 to 134.
 
 #include "common.hpp"
 
@@ -957,7 +964,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
 
 // Logits a row may have: its chunks have to fit the bins, and the list.
 constexpr int64_t kMaxVocab = 500000;
-// A block of 1024 threads per row while every row gets a CU of its own.
+// A block of 1024 threads per row while every row gets a CU of its own (256 rows with top-p: 40 us); smaller
+// blocks gain only where two share a CU (1000 rows: 127 against 155 us).
 constexpr int64_t kRowsAtOnce = 256;
 static_assert(kMaxVocab + 8 <= (int64_t)kBins * kWave * 4 - kMostWaves * kWave * 4, "a bin per chunk");
 
