@@ -432,7 +432,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
   int cut_index = -1;
   bool cutting = false; // (there is a cut at all)
   auto in_front = [&](float x, int index) __attribute__((always_inline)) {
-    return x > cut || (x == cut && index <= cut_index);
+    return (x > cut) | ((x == cut) & (index <= cut_index)); // (no branch)
   };
   const double min_mass = a.min_p.at(row);
   if (min_mass > 0.0) {
@@ -767,13 +767,20 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     const uint32_t beside = kBins + lane; // (what the steps do not hold goes here, a place per lane)
     __syncthreads();
     for_chunks([&](int c, const V &v) __attribute__((always_inline)) {
+      float x[kVec];
+      uint32_t step[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) x[e] = static_cast<float>(v[e]);
+      if (cutting)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) x[e] = in_front(x[e], first_of(c, at_lane) + e) ? x[e] : -INFINITY;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        float x = static_cast<float>(v[e]);
-        if (cutting && !in_front(x, first_of(c, at_lane) + e)) x = -INFINITY;
-        const uint32_t step = (uint32_t)fminf((top - x) * per_step, (float)(kBins + kWave));
-        atomicAdd(&lds.counts[step < beside ? step : beside], 1u);
+        step[e] = (uint32_t)fminf((top - x[e]) * per_step, (float)(kBins + kWave));
+        step[e] = step[e] < beside ? step[e] : beside;
       }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) atomicAdd(&lds.counts[step[e]], 1u);
     });
     __syncthreads();
     // (2^40 to the largest mass, each taken at the middle of its step)
@@ -844,7 +851,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
           const u64 bits = __builtin_bit_cast(u64, w[e]);
           const uint32_t upper = x[e] > sure_x ? (uint32_t)(bits >> 32) : 0u;
           kept += __builtin_bit_cast(double, (u64)upper << 32 | (uint32_t)bits);
-          near |= x[e] >= window_x && x[e] <= sure_x;
+          near |= (x[e] >= window_x) & (x[e] <= sure_x);
         }
         if (near)
 #pragma unroll
