@@ -19,7 +19,7 @@
 //
 // One block takes a row, 1024 threads and a CU for itself up to 256 rows; beyond that
 // 512, two to a CU, one waiting for memory or at a barrier while the other computes
-// (1000 rows of 50257 fp32 logits with top-p: 127 against 155 us). It holds the row in
+// (1000 rows of 50257 fp32 logits with top-p: 127 against 155 us when this was chosen, 120 now). It holds the row in
 // registers and LDS (53248 logits of 32 bits, or 20480, twice that in 16 bits; what exceeds them
 // is read again, ahead of its use), each wave a run of it. Such a row is read in 5 to 8 us; what
 // costs the time then is arithmetic, one operation in 64 bits after another, and
@@ -40,7 +40,7 @@
 //    chunk, which all waves sum together, and looks inside that.
 // Windows too full for the list (equal logits by the thousand) are searched by
 // histograms over the bits of the logits. Measured, us a call: one row of 50257 fp32 logits, top-k 50 and
-// top-p, 12.6; 256 rows in bf16, settings of their own, 39; 1000 rows in fp32, top-p 0.92, 127 to 134.
+// top-p, 12.6; 256 rows in bf16, settings of their own, 39; 1000 rows in fp32, top-p 0.92, 120 to 130.
 
 #include "common.hpp"
 

@@ -733,16 +733,40 @@ _HALVES = (torch.float16, torch.bfloat16)
 _Strides = {n: ctypes.c_int64 * n for n in (2, 4, 8, 16)}
 
 
-def _packed_strided(t):
-    """t [T, heads, D] as the kernels over packed tokens can read it; a copy if not."""
-    if t.is_contiguous():
-        return t if t.data_ptr() % 16 == 0 else t.clone()
+def _stream_of(device):
+    """torch's current stream on the device of that index, as the library's stream argument."""
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def _device_scope(device):
+    return _NO_SWITCH if device == _current_device() else torch.cuda.device(device)
+
+
+def _packed_view(t):
+    """t [T, heads, D] as the kernels over packed tokens can read it (a copy if they
+    cannot): the tensor, its pointer, its head and token strides."""
+    pointer = t.data_ptr()
     st, sh, sd = t.stride()
-    ok = sd == 1 and st % 8 == 0 and sh % 8 == 0 and st >= t.shape[2] and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
+    if sd != 1 or (st | sh) & 7 or pointer & 15 or st < t.shape[2]:
+        t = t.clone(memory_format=torch.contiguous_format)
+        pointer = t.data_ptr()
+        st, sh, _ = t.stride()
+    return t, pointer, sh, st
 
 
 def _packed_args(query, key, value, packed):
+    """The checks of a call over packed tokens; the dtype code and the device's index."""
+    try:  # a call that is right, with as little work as can be
+        device, dtype, shape = query.get_device(), query.dtype, key.shape
+        t, h, d = query.shape
+        tk, hkv, dk = shape
+        if (device >= 0 and key.get_device() == device and value.get_device() == device
+                and packed.blocks.get_device() == device and dtype in _HALVES and key.dtype is dtype
+                and value.dtype is dtype and value.shape == shape and tk == t and dk == d and hkv and h % hkv == 0
+                and d in PREFILL_HEAD_DIMS and packed.total <= t):
+            return _DTYPE[dtype], device
+    except (AttributeError, ValueError):
+        pass
     _device_tensor(query, "query")
     _device_tensor(key, "key", query)
     _device_tensor(value, "value", query)
@@ -765,20 +789,12 @@ def _packed_args(query, key, value, packed):
         raise RuntimeError(f"the sequences have {packed.total} tokens, the tensors {t}")
     if packed.blocks.device != query.device:
         raise RuntimeError(f"the sequences are on {packed.blocks.device}, query on {query.device}")
-    return code
+    return code, query.get_device()
 
 
 @functools.lru_cache(maxsize=256)
 def _strides_of(*flat):
     return _Strides[len(flat)](*flat)
-
-
-def _token_strides(*tensors):
-    flat = []
-    for t in tensors:
-        st, sh, _ = t.stride()
-        flat += (sh, st)
-    return _strides_of(*flat)
 
 
 @functools.lru_cache(maxsize=256)
@@ -801,26 +817,28 @@ def attention_packed_forward(query, key, value, packed, scale, window=0, want_ls
     [T, H, D] (rows behind the last sequence: zeros), with ``want_lse`` also what
     ``attention_packed_backward`` takes: the part of the output that its
     rounding left out, [T, H, D], and the fp32 [H, T] log2-sum-exp."""
-    code = _packed_args(query, key, value, packed)
+    code, device = _packed_args(query, key, value, packed)
     t, h, d = query.shape
-    q, k, v = _packed_strided(query), _packed_strided(key), _packed_strided(value)
+    q, qp, qh, qt = _packed_view(query)
+    k, kp, kh, kt = _packed_view(key)
+    v, vp, vh, vt = _packed_view(value)
     out = _packed_empty(t, h, d, packed, query)
     low = torch.empty((t, h, d), dtype=query.dtype, device=query.device) if want_lse else None
     lse = torch.empty((h, t), dtype=torch.float32, device=query.device) if want_lse else None
     if packed.total and h:
         blocks = packed.blocks
-        with _on_device(q):
+        with _device_scope(device):
             _lib.check(_lib.load().oslo_attention_packed_fwd(
-                out.data_ptr(), _ptr(low), _ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(),
-                blocks.shape[1], scale, t, packed.max_length, h, k.shape[1], d, window, _token_strides(q, k, v, out),
-                code, _stream(q)))
+                out.data_ptr(), _ptr(low), _ptr(lse), qp, kp, vp, blocks.data_ptr(), blocks.shape[1], scale, t,
+                packed.max_length, h, key.shape[1], d, window, _strides_of(qh, qt, kh, kt, vh, vt, d, h * d), code,
+                _stream_of(device)))
     return (out, low, lse) if want_lse else out
 
 
 def attention_packed_backward(grad_out, query, key, value, out, out_low, lse, packed, scale, window=0):
     """Gradients of ``attention_packed_forward`` with respect to query, key and
     value (dense; rows behind the last sequence: zeros)."""
-    code = _packed_args(query, key, value, packed)
+    code, device = _packed_args(query, key, value, packed)
     for what, x in (("grad_out", grad_out), ("out", out), ("out_low", out_low)):
         _device_tensor(x, what, query)
         if x.shape != query.shape or x.dtype != query.dtype:
@@ -831,7 +849,8 @@ def attention_packed_backward(grad_out, query, key, value, out, out_low, lse, pa
     _require(lse.dtype == torch.float32 and tuple(lse.shape) == (h, t) and lse.is_contiguous(),
              "lse must be the fp32 [H, T] tensor of the forward")
     _require(out.is_contiguous() and out_low.is_contiguous(), "out and out_low must be the forward's")
-    q, k, v, o, g = (_packed_strided(x) for x in (query, key, value, out, grad_out))
+    views = [_packed_view(x) for x in (query, key, value, out, grad_out)]
+    (_, qp, *_), (_, kp, *_), (_, vp, *_), (_, op, *_), (_, gp, *_) = views
     dq = _packed_empty(t, h, d, packed, query)
     dk, dv = (_packed_empty(t, hkv, d, packed, query) for _ in range(2))
     if packed.total and h:
@@ -839,16 +858,22 @@ def attention_packed_backward(grad_out, query, key, value, out, out_low, lse, pa
         split, parts = packed.shared_blocks(h, hkv, d, window)
         ws = torch.empty(lib.oslo_attention_packed_bwd_workspace_bytes(t, h, hkv, d, split, parts) // 4,
                          dtype=torch.float32, device=query.device)
-        with _on_device(q):
+        strides = [n for _, _, sh, st in views for n in (sh, st)] + [d, h * d, d, hkv * d, d, hkv * d]
+        with _device_scope(device):
             _lib.check(lib.oslo_attention_packed_bwd(
-                _ptr(dq), _ptr(dk), _ptr(dv), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(o),
-                _ptr(out_low), _ptr(lse), _ptr(ws), _ptr(packed.blocks[0]), _ptr(packed.blocks[1]),
-                packed.blocks.shape[1], split, parts, scale, t,
-                packed.max_length, h, hkv, d, window, _token_strides(q, k, v, o, g, dq, dk, dv), code, _stream(q)))
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), gp, qp, kp, vp, op, out_low.data_ptr(), lse.data_ptr(),
+                ws.data_ptr(), packed.blocks[0].data_ptr(), packed.blocks[1].data_ptr(), packed.blocks.shape[1], split,
+                parts, scale, t, packed.max_length, h, hkv, d, window, _strides_of(*strides), code, _stream_of(device)))
     return dq, dk, dv
 
 
 def _index_tensor(t, what, like, length):
+    try:
+        if (t.get_device() == like.get_device() and t.dtype is torch.int32 and t.shape == (length,)
+                and t.is_contiguous()):
+            return t
+    except AttributeError:
+        pass
     _device_tensor(t, what, like)
     if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != length:
         raise RuntimeError(f"{what} must be int32 [{length}]")
@@ -857,15 +882,20 @@ def _index_tensor(t, what, like, length):
 
 def _cache_args(cache, like, what):
     """What every call over a ``PagedKV`` passes on: its pointers and sizes."""
-    keys = cache.key_pages
-    if keys.device != like.device:
+    keys, key_scales = cache.key_pages, cache.key_scales
+    dtype = like.dtype
+    if keys.get_device() != like.get_device():
         raise RuntimeError(f"the cache is on {keys.device}, {what} on {like.device}")
-    if like.dtype not in _HALVES:
-        raise RuntimeError(f"{what}: fp16 or bf16, got {like.dtype}")
-    pointers = (keys.data_ptr(), cache.value_pages.data_ptr(), _ptr(cache.key_scales), _ptr(cache.value_scales))
-    if not cache.quantized and keys.dtype != like.dtype:
-        raise RuntimeError(f"{what} is {like.dtype}, the cache {keys.dtype}")
-    return pointers, (*cache.table.shape, keys.shape[0]), keys.shape[1:]
+    if dtype not in _HALVES:
+        raise RuntimeError(f"{what}: fp16 or bf16, got {dtype}")
+    if key_scales is None:
+        if keys.dtype is not dtype:
+            raise RuntimeError(f"{what} is {dtype}, the cache {keys.dtype}")
+        pointers = keys.data_ptr(), cache.value_pages.data_ptr(), None, None
+    else:
+        pointers = keys.data_ptr(), cache.value_pages.data_ptr(), key_scales.data_ptr(), cache.value_scales.data_ptr()
+    pages, *sizes = keys.shape
+    return pointers, (*cache.table.shape, pages), sizes
 
 
 def paged_kv_write(cache, key, value, sequence, position):
@@ -882,11 +912,13 @@ def paged_kv_write(cache, key, value, sequence, position):
         raise RuntimeError("key and value differ in shape or dtype")
     t = key.shape[0]
     sequence, position = _index_tensor(sequence, "sequence", key, t), _index_tensor(position, "position", key, t)
-    k, v = _packed_strided(key), _packed_strided(value)
-    with _on_device(k):
+    k, kp, kh, kt = _packed_view(key)
+    v, vp, vh, vt = _packed_view(value)
+    device = key.get_device()
+    with _device_scope(device):
         _lib.check(_lib.load().oslo_paged_kv_write(
-            *pointers, k.data_ptr(), v.data_ptr(), sequence.data_ptr(), position.data_ptr(), cache.table.data_ptr(), t,
-            *counts, hkv, page, d, _token_strides(k, v), code, _stream(k)))
+            *pointers, kp, vp, sequence.data_ptr(), position.data_ptr(), cache.table.data_ptr(), t, *counts, hkv, page, d,
+            _strides_of(kh, kt, vh, vt), code, _stream_of(device)))
 
 
 def paged_kv_read(cache, sequence, position, dtype):
@@ -901,10 +933,11 @@ def paged_kv_read(cache, sequence, position, dtype):
     key, value = (torch.empty((t, hkv, d), dtype=dtype, device=sequence.device) for _ in range(2))
     code = _dtype_code(key, "dtype")
     pointers, counts, _ = _cache_args(cache, key, "dtype")
-    with _on_device(key):
+    device = key.get_device()
+    with _device_scope(device):
         _lib.check(_lib.load().oslo_paged_kv_read(
             key.data_ptr(), value.data_ptr(), *pointers, sequence.data_ptr(), position.data_ptr(),
-            cache.table.data_ptr(), t, *counts, hkv, page, d, code, _stream(key)))
+            cache.table.data_ptr(), t, *counts, hkv, page, d, code, _stream_of(device)))
     return key, value
 
 
@@ -928,14 +961,14 @@ def attention_paged_decode_forward(query, cache, lengths, scale, window=0):
     if qd != 1 or qb % 8 or qh % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         qb, qh, _ = q.stride()
-    lib = _lib.load()
     floats = _decode_workspace_floats(b, h, hkv, d, counts[1] * page, window)
     ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     out = q.new_empty((b, h, d))
-    with _on_device(q):
-        _lib.check(lib.oslo_attention_paged_decode_fwd(
+    device = q.get_device()
+    with _device_scope(device):
+        _lib.check(_lib.load().oslo_attention_paged_decode_fwd(
             out.data_ptr(), q.data_ptr(), *pointers, cache.table.data_ptr(), lengths.data_ptr(), _ptr(ws), scale,
-            *counts, h, hkv, page, d, window, _strides_of(qb, qh), code, _stream(q)))
+            *counts, h, hkv, page, d, window, _strides_of(qb, qh), code, _stream_of(device)))
     return out
 
 
@@ -970,11 +1003,12 @@ def sample_forward(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=
     uniforms = uniforms.contiguous()
     tokens = x.new_empty((rows,), dtype=torch.int64)
     logprobs = uniforms.new_empty((rows,))
-    with _on_device(x):
+    device = x.get_device()
+    with _device_scope(device):
         _lib.check(_lib.load().oslo_sample(
             tokens.data_ptr(), logprobs.data_ptr(), x.data_ptr(), uniforms.data_ptr(), _ptr(temperature),
             temperature_all, _ptr(top_k), int(top_k_all), _ptr(top_p), top_p_all, _ptr(min_p), min_p_all, rows, vocab,
-            x.stride(0), code, _stream(x)))
+            x.stride(0), code, _stream_of(device)))
     return tokens, logprobs
 
 
