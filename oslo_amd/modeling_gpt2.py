@@ -292,6 +292,11 @@ class GPT2Block(nn.Module):
         self.ln_2 = nn.LayerNorm(config.hidden_size, eps=config.layer_norm_epsilon)
         self.mlp = GPT2MLP(inner, config)
 
+    @property
+    def takes_sequences(self):
+        """The attention knows a ``SequenceLayer`` in the place of a past."""
+        return isinstance(self.attn, FusedGPT2Attention)
+
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         a = self.attn(self.ln_1(hidden_states), layer_past=layer_past, attention_mask=attention_mask,
                       head_mask=head_mask, use_cache=use_cache)
@@ -306,8 +311,6 @@ class FusedGPT2Block(GPT2Block):
     No counterpart in the reference, which fuses attention and MLP only
     (oslo/models/gpt2/configuration_gpt2.py:272-284); the arithmetic is that
     of oslo/models/gpt2/modeling_gpt2.py:420-481."""
-
-    takes_sequences = True
 
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         if not (isinstance(self.attn, FusedGPT2Attention) and isinstance(self.mlp, FusedGPT2MLP)):

@@ -300,6 +300,11 @@ class GPTNeoBlock(nn.Module):
         self.ln_2 = nn.LayerNorm(config.hidden_size, eps=config.layer_norm_epsilon)
         self.mlp = GPTNeoMLP(inner, config)
 
+    @property
+    def takes_sequences(self):
+        """The attention knows a ``SequenceLayer`` in the place of a past."""
+        return isinstance(self.attn.attention, FusedGPTNeoSelfAttention)  # (local layers too)
+
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         a = self.attn(self.ln_1(hidden_states), layer_past=layer_past, attention_mask=attention_mask,
                       head_mask=head_mask, use_cache=use_cache)
@@ -314,8 +319,6 @@ class FusedGPTNeoBlock(GPTNeoBlock):
     No counterpart in the reference, which fuses attention and MLP only
     (oslo/models/gpt_neo/configuration_gpt_neo.py:330-342); the arithmetic is
     that of oslo/models/gpt_neo/modeling_gpt_neo.py:333-380."""
-
-    takes_sequences = True
 
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         inner = self.attn.attention

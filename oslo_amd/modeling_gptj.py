@@ -328,6 +328,11 @@ class GPTJBlock(nn.Module):
         self.attn = GPTJAttention(config)
         self.mlp = GPTJMLP(inner, config)
 
+    @property
+    def takes_sequences(self):
+        """The attention knows a ``SequenceLayer`` in the place of a past."""
+        return isinstance(self.attn, FusedGPTJAttention)
+
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         residual = hidden_states
         hidden_states = self.ln_1(hidden_states)
@@ -351,8 +356,6 @@ class FusedGPTJBlock(GPTJBlock):
     their last projections instead (attention output + residual first, the
     feed-forward output on top). No counterpart in the reference, which fuses
     attention and MLP only (oslo/models/gptj/configuration_gptj.py:155-167)."""
-
-    takes_sequences = True
 
     def forward(self, hidden_states, layer_past=None, attention_mask=None, head_mask=None, use_cache=False):
         if not (isinstance(self.attn, FusedGPTJAttention) and isinstance(self.mlp, FusedGPTJMLP)):

@@ -254,7 +254,7 @@ def sequence_positions(past_key_values, input_ids, limit, blocks):
     model knows (None: any)."""
     if past_key_values is None or not isinstance(past_key_values[0], SequenceLayer):
         return None
-    if not hasattr(blocks[0], "takes_sequences"):
+    if not all(block.takes_sequences for block in blocks):
         raise RuntimeError("sequences of different lengths need the fused modules: call model.fuse() first")
     if input_ids.dim() != 2 or input_ids.size(0) != 1:
         raise ValueError("sequences of different lengths are one row of tokens: input_ids must be [1, tokens]")

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from oslo_amd import GPT2Config, GPT2LMHeadModel, PackedSequences, PagedKV, PagedState, kernels
+from oslo_amd import GPT2Config, GPT2LMHeadModel, GPTNeoConfig, GPTNeoForCausalLM, PackedSequences, PagedKV, PagedState, kernels
 from oslo_amd import _lib
 from oslo_amd.sequences import packed_labels, sequence_layers
 
@@ -228,6 +228,11 @@ def test_models_refuse_what_sequences_do_not_take():
         model(row[:, :5], packed=packed)
     with pytest.raises(RuntimeError, match="drop"):
         model.train()(row, packed=packed)
+    from oslo_amd.modeling_gpt_neo import GPTNeoSelfAttention
+    half = GPTNeoForCausalLM(GPTNeoConfig(vocab_size=11, max_position_embeddings=8, hidden_size=64, num_layers=2, num_heads=1))
+    half.fuse(modules=[GPTNeoSelfAttention])  # (its local layers are not)
+    with pytest.raises(RuntimeError, match="fuse"):
+        half.eval()(row, packed=packed)
 
 
 def test_generate_refuses_what_sampling_and_lists_do_not_take():
