@@ -51,7 +51,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 def _stream(t):
     """torch's current stream on t's device, as the library's stream argument."""
     if _raw_stream is not None:
-        return _raw_stream(t.device.index)
+        return ctypes.c_void_p(_raw_stream(t.device.index))
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
