@@ -738,12 +738,17 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
     walk();
   }
 
-  if (own >= S) return;
+  // PACKED: the gradients leave through the wave's part of LDS, in whole rows. (Straight from the accumulators a
+  // store is 16 bytes of 32 rows, and the blocks of short walks, which a window makes, sent two thirds of
+  // the cache's requests that way.)
+  if constexpr (PACKED) __syncthreads(); // every wave has read its last operands
+  else if (own >= S) return;
   typedef T Out4 __attribute__((ext_vector_type(4)));
   auto store = [&](const f32x16 (&sums)[kBlocksD], void *out_base, const Strides3 &st_out, float factor)
                    __attribute__((always_inline)) {
     if constexpr (PACKED && kKeysOwn) {
       if (part_slot >= 0) {
+        if (own >= S) return;
         float *fp = a.partial + ((part_slot * 2 + (out_base == a.dv ? 1 : 0)) * kOwnPerBlock + 32 * wave + col) * (int64_t)D;
 #pragma unroll
         for (int i = 0; i < kBlocksD; ++i)
@@ -754,6 +759,33 @@ __global__ __launch_bounds__(kBlockThreads, bwd_blocks_per_cu(D, ROLE)) void att
                             sums[i][4 * j + 3] * factor);
         return;
       }
+    }
+    if constexpr (PACKED) {
+      constexpr int kRow = D + 8, kRowLanes = D / 8; // (rows 16 bytes apart in the banks)
+      static_assert(4 * 32 * kRow <= 2 * kSchedBuffers * kTile, "the tiles' place holds the four waves' rows");
+      T *const mine = o1_lds + wave * (32 * kRow);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); // (the rows of the gradient before have been read)
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < kBlocksD; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          Out4 w;
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) w[tt] = static_cast<T>(sums[i][4 * j + tt] * factor);
+          *reinterpret_cast<Out4 *>(mine + col * kRow + 32 * i + 8 * j + 4 * half) = w;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      T *const rows = static_cast<T *>(out_base) + (kKeysOwn ? kv_hd : hd) * st_out.h + (start + wave_own0) * st_out.s;
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += kWave / kRowLanes) {
+        const int r = r0 + lane / kRowLanes, at = 8 * (lane % kRowLanes);
+        const Frag w = *reinterpret_cast<const Frag *>(mine + r * kRow + at);
+        if (wave_own0 + r < S) *reinterpret_cast<Frag *>(rows + r * st_out.s + at) = w;
+      }
+      return;
     }
     T *op = static_cast<T *>(out_base) + b * st_out.b + (kKeysOwn ? kv_hd : hd) * st_out.h + (start + own) * st_out.s;
 #pragma unroll
