@@ -13,9 +13,9 @@
 // several blocks, each with some heads of the group, whose fp32 sums a last kernel
 // adds in order: 575 us become 460 to 500 for the dK/dV pass there (355 Gflop, 0.74
 // Pflop/s), and 9 us go into the last kernel; the dQ pass takes 295 (267 Gflop, 0.9).
-// With a window of 256 (8794 tokens, 20 heads) the passes take 90 and 151 us, half of it
-// for what a block reads and writes before and after its 12 tiles: 7.7 us a tile over
-// both passes, 127 us for the rest, which at one block per CU nothing hides.
+// With a window of 256 (8794 tokens, 20 heads) the passes take 84 and 137 us, half of it
+// for what a block reads and writes before and after its 12 tiles: 7.9 us a tile over
+// both passes, 112 us for the rest, which at one block per CU nothing hides.
 //
 // Two lists of the same entries: the dQ pass wants the blocks with the most keys first,
 // the others those with the most queries left.

@@ -848,7 +848,9 @@ class FusedSampling(object):
 
     @staticmethod
     def apply(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-        return get_custom_kernels().sample_forward(logits.detach(), uniforms, temperature, top_k, top_p, min_p)
+        if logits.requires_grad:
+            logits = logits.detach()
+        return get_custom_kernels().sample_forward(logits, uniforms, temperature, top_k, top_p, min_p)
 
 
 class FusedLinearRows(object):

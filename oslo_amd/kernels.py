@@ -822,7 +822,10 @@ def attention_packed_forward(query, key, value, packed, scale, window=0, want_ls
     q, qp, qh, qt = _packed_view(query)
     k, kp, kh, kt = _packed_view(key)
     v, vp, vh, vt = _packed_view(value)
-    out = _packed_empty(t, h, d, packed, query)
+    if q is query and qh == d and qt == h * d and packed.total == t:
+        out = torch.empty_like(query)  # (the quicker way to the same)
+    else:
+        out = _packed_empty(t, h, d, packed, query)
     low = torch.empty((t, h, d), dtype=query.dtype, device=query.device) if want_lse else None
     lse = torch.empty((h, t), dtype=torch.float32, device=query.device) if want_lse else None
     if packed.total and h:
@@ -963,7 +966,7 @@ def attention_paged_decode_forward(query, cache, lengths, scale, window=0):
         qb, qh, _ = q.stride()
     floats = _decode_workspace_floats(b, h, hkv, d, counts[1] * page, window)
     ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    out = q.new_empty((b, h, d))
+    out = torch.empty_like(q) if qh == d and qb == h * d else q.new_empty((b, h, d))
     device = q.get_device()
     with _device_scope(device):
         _lib.check(_lib.load().oslo_attention_paged_decode_fwd(
@@ -1001,8 +1004,8 @@ def sample_forward(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=
     min_p, min_p_all = _row_setting(min_p, "min_p", torch.float32, rows, logits)
     x = logits if logits.stride(1) == 1 else logits.contiguous()
     uniforms = uniforms.contiguous()
-    tokens = x.new_empty((rows,), dtype=torch.int64)
-    logprobs = uniforms.new_empty((rows,))
+    tokens = torch.empty_like(uniforms, dtype=torch.int64)
+    logprobs = torch.empty_like(uniforms)
     device = x.get_device()
     with _device_scope(device):
         _lib.check(_lib.load().oslo_sample(
