@@ -197,3 +197,22 @@ def test_many_rows_draw_as_few_do(vocab, dtype):
         few = [FusedSampling.apply(logits[i:i + 130], u[i:i + 130], **kw) for i in (0, 130)]
         assert torch.equal(many[0], torch.cat([t for t, _ in few])), kw
         assert torch.equal(many[1], torch.cat([p for _, p in few])), kw
+
+
+@pytest.mark.parametrize("vocab", [1001, 50257])
+def test_logits_as_far_apart_as_the_type_allows(vocab):
+    """Differences that overflow 32 bits, in rows that begin anywhere, with and without nothing but -inf beside."""
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn((4, vocab), generator=g)
+    logits[0] *= 1.0e38
+    logits[0].clamp_(-3.4e38, 3.4e38)
+    logits[1, ::7] = -3.4e38
+    logits[1, 3] = 3.4e38
+    logits[2] = -3.4e38
+    logits[2, ::2] = float("-inf")
+    logits[3] = float("-inf")
+    logits[3, 11:400] = torch.randn(389, generator=g)
+    logits, u = logits.to(DEV), torch.rand(4, generator=g).to(DEV)
+    for kw in (dict(), dict(top_k=5), dict(top_k=300), dict(top_k=900, top_p=0.7), dict(top_p=0.9), dict(min_p=0.2),
+               dict(top_k=50, temperature=1.0e37), dict(top_p=0.5, temperature=1.0e-37)):
+        check(logits, u, **kw)
