@@ -618,9 +618,9 @@ size_t oslo_attention_packed_bwd_workspace_bytes(int64_t tokens, int64_t heads,
 
 /*
  * Gradients of the packed attention from dout, the inputs, the forward's out,
- * out_low (or NULL: less exact where few keys carry a row) and lse: the formulas of oslo_attention_prefill_bwd per sequence; dk and dv are
- * summed over the query heads of a group in fp32, in a fixed order, and rounded
- * once. query_blocks and key_blocks hold the same entries as the forward's
+ * out_low (or NULL: less exact where few keys carry a row) and lse: the formulas
+ * of oslo_attention_prefill_bwd per sequence; dk and dv are summed over the query
+ * heads of a group in fp32, in a fixed order, and rounded once. query_blocks and key_blocks hold the same entries as the forward's
  * `blocks` (most keys first, and most queries left first, run fastest).
  * The work on the first `split` entries of key_blocks is shared by `parts` blocks
  * each, which take the heads of a group between them (1 <= parts <= heads /
@@ -741,8 +741,8 @@ int oslo_attention_paged_decode_fwd(void *out, const void *q,
  * token -1 and -inf. Uniforms outside [0, 1) are taken to its nearest end.
  * Every setting is a number of the call or, where the pointer is given, one per
  * row (fp32, top_k int32). Masses are summed as whole multiples of
- * 2^(ceil(log2 vocab) - 62) of the largest: the token does not depend on the order of
- * a sum. vocab up to 500000. No workspace.
+ * 2^(ceil(log2 vocab) - 61), at least 2^-49, of the largest: the token does not
+ * depend on the order of a sum. vocab up to 500000. No workspace.
  * The reference samples on the framework's operators after sorting
  * (oslo/generation_utils.py).
  */

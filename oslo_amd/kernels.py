@@ -802,6 +802,11 @@ def _decode_workspace_floats(*sizes):
     return _lib.load().oslo_attention_paged_decode_workspace_bytes(*sizes) // 4
 
 
+@functools.lru_cache(maxsize=256)
+def _packed_workspace_floats(*sizes):
+    return _lib.load().oslo_attention_packed_bwd_workspace_bytes(*sizes) // 4
+
+
 def _packed_empty(tokens, heads, d, packed, like):
     """An uninitialised [tokens, heads, D] whose rows behind the last sequence are zeros."""
     out = like.new_empty((tokens, heads, d))
@@ -826,7 +831,7 @@ def attention_packed_forward(query, key, value, packed, scale, window=0, want_ls
         out = torch.empty_like(query)  # (the quicker way to the same)
     else:
         out = _packed_empty(t, h, d, packed, query)
-    low = torch.empty((t, h, d), dtype=query.dtype, device=query.device) if want_lse else None
+    low = torch.empty_like(out) if want_lse else None
     lse = torch.empty((h, t), dtype=torch.float32, device=query.device) if want_lse else None
     if packed.total and h:
         blocks = packed.blocks
@@ -842,12 +847,13 @@ def attention_packed_backward(grad_out, query, key, value, out, out_low, lse, pa
     """Gradients of ``attention_packed_forward`` with respect to query, key and
     value (dense; rows behind the last sequence: zeros)."""
     code, device = _packed_args(query, key, value, packed)
+    shape, dtype = query.shape, query.dtype
     for what, x in (("grad_out", grad_out), ("out", out), ("out_low", out_low)):
         _device_tensor(x, what, query)
-        if x.shape != query.shape or x.dtype != query.dtype:
+        if x.shape != shape or x.dtype is not dtype:
             raise RuntimeError(f"{what} must be like query")
     _device_tensor(lse, "lse", query)
-    t, h, d = query.shape
+    t, h, d = shape
     hkv = key.shape[1]
     _require(lse.dtype == torch.float32 and tuple(lse.shape) == (h, t) and lse.is_contiguous(),
              "lse must be the fp32 [H, T] tensor of the forward")
@@ -857,16 +863,15 @@ def attention_packed_backward(grad_out, query, key, value, out, out_low, lse, pa
     dq = _packed_empty(t, h, d, packed, query)
     dk, dv = (_packed_empty(t, hkv, d, packed, query) for _ in range(2))
     if packed.total and h:
-        lib = _lib.load()
         split, parts = packed.shared_blocks(h, hkv, d, window)
-        ws = torch.empty(lib.oslo_attention_packed_bwd_workspace_bytes(t, h, hkv, d, split, parts) // 4,
-                         dtype=torch.float32, device=query.device)
+        ws = lse.new_empty((_packed_workspace_floats(t, h, hkv, d, split, parts),))
+        blocks, num_blocks = packed.blocks.data_ptr(), packed.blocks.shape[1]  # two lists of 16-byte entries
         strides = [n for _, _, sh, st in views for n in (sh, st)] + [d, h * d, d, hkv * d, d, hkv * d]
         with _device_scope(device):
-            _lib.check(lib.oslo_attention_packed_bwd(
+            _lib.check(_lib.load().oslo_attention_packed_bwd(
                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), gp, qp, kp, vp, op, out_low.data_ptr(), lse.data_ptr(),
-                ws.data_ptr(), packed.blocks[0].data_ptr(), packed.blocks[1].data_ptr(), packed.blocks.shape[1], split,
-                parts, scale, t, packed.max_length, h, hkv, d, window, _strides_of(*strides), code, _stream_of(device)))
+                ws.data_ptr(), blocks, blocks + 16 * num_blocks, num_blocks, split, parts, scale, t, packed.max_length, h,
+                hkv, d, window, _strides_of(*strides), code, _stream_of(device)))
     return dq, dk, dv
 
 
