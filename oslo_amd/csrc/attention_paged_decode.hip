@@ -636,6 +636,8 @@ __global__ __launch_bounds__(kBlockThreads) void attention_paged_join_kernel(con
 //   64 features x 12 heads:  1 x 300 positions 4.4 (7.4), 4 x 300 5.7 (8.0), 32 x 1024 15.2 (16.3), 400 x 1024 111 (122);
 //   128 x 8, 32 query heads: 4 x 512 7.8 (8.9), 4 x 1024 14.2 (10.5), 32 x 1024 19.6 (22.5), 32 x 2048 33 (31);
 //   256 x 16:                4 x 256 7.7 (9.8), 1 x 512 13.7 (8.8), 16 x 512 17.7 (19.2), 32 x 2048 116 (95).
+// (Asked for all sequences of a call, not for those of one of its launches: the workspace
+// has to fit every launch.)
 inline int64_t meet_tiles(int64_t blocks, int64_t head_dim) { return blocks >= 256 ? 32 : head_dim == 256 ? 8 : 16; }
 
 // The grid: as many blocks as fit the card's 256 CUs at a time, or fewer where the
@@ -647,14 +649,15 @@ struct DecodeGrid {
   bool join;              // some sequence may have more than one
   bool meet;              // a block takes a whole sequence
 };
-inline DecodeGrid decode_grid(int64_t sequences, int64_t kv_heads, int64_t column_groups, int64_t head_dim,
+// `sequences` of the `all` of a call.
+inline DecodeGrid decode_grid(int64_t sequences, int64_t all, int64_t kv_heads, int64_t column_groups, int64_t head_dim,
                               int64_t max_length, int64_t window) {
   // (a window may begin anywhere in its first tile)
   const int64_t span = window > 0 && window < max_length ? std::min(window + kTileKeys - 1, max_length) : max_length;
   const int64_t per_sequence = std::max<int64_t>(1, (span + kMinChunk - 1) / kMinChunk);
   const int64_t slots = kv_heads * column_groups;
   DecodeGrid g;
-  g.meet = per_sequence > 1 && per_sequence <= meet_tiles(sequences * slots, head_dim);
+  g.meet = per_sequence > 1 && per_sequence <= meet_tiles(all * slots, head_dim);
   if (g.meet) {
     g.blocks = sequences * slots;
     g.chunks = 0;
@@ -681,7 +684,7 @@ int launch_paged_decode(PagedDecodeArgs a, int64_t max_length, hipStream_t strea
     part.lengths = a.lengths + s0;
     part.q = static_cast<const T *>(a.q) + s0 * a.q_seq;
     part.out = static_cast<T *>(a.out) + s0 * a.heads * D;
-    const DecodeGrid grid = decode_grid(n, a.map.kv_heads, a.column_groups, D, max_length, a.window);
+    const DecodeGrid grid = decode_grid(n, sequences, a.map.kv_heads, a.column_groups, D, max_length, a.window);
     const int64_t slots = (int64_t)a.map.kv_heads * a.column_groups;
     part.full_chunks = (double)full_chunks(kWavesPerBlock * grid.blocks, n * slots) / (double)slots;
     part.plan = grid.join ? reinterpret_cast<int *>(a.partial) : nullptr;
@@ -724,7 +727,7 @@ extern "C" size_t oslo_attention_paged_decode_workspace_bytes(int64_t sequences,
   if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_length <= 0 || heads % kv_heads) return 0;
   const int64_t groups = (heads / kv_heads + kColumns - 1) / kColumns;
   const int64_t n = std::min<int64_t>(sequences, kMaxSequences); // (of one launch)
-  const DecodeGrid g = decode_grid(n, kv_heads, groups, head_dim, max_length, window);
+  const DecodeGrid g = decode_grid(n, sequences, kv_heads, groups, head_dim, max_length, window);
   if (!g.join) return 0;
   return ((size_t)plan_ints(n) + (size_t)g.chunks * (size_t)heads * (size_t)(head_dim + 4)) * sizeof(float);
 }
@@ -762,7 +765,7 @@ extern "C" int oslo_attention_paged_decode_fwd(void *out, const void *q, const v
   const int64_t max_length = max_pages * page_size;
   a.group = (int)(heads / kv_heads);
   a.column_groups = (a.group + kColumns - 1) / kColumns;
-  if (!workspace && decode_grid(std::min<int64_t>(sequences, kMaxSequences), kv_heads, a.column_groups, head_dim,
+  if (!workspace && decode_grid(std::min<int64_t>(sequences, kMaxSequences), sequences, kv_heads, a.column_groups, head_dim,
                                 max_length, window).join)
     return fail(OSLO_E_BAD_ARG, "%s: null workspace", name);
   if (!aligned16(workspace)) return fail(OSLO_E_UNSUPPORTED, "%s: the workspace must be 16-byte aligned", name);

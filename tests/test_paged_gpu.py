@@ -229,6 +229,18 @@ def test_decode_of_many_sequences(count, longest, window, eight):
     assert not out[n == 0].any()
 
 
+def test_the_last_launch_of_many_sequences_is_of_the_calls_kind():
+    """4096 sequences in one launch, a block each; one more, of a thousand positions, in a second."""
+    lengths = torch.randint(0, 41, (4097,), generator=torch.Generator().manual_seed(1)).tolist()
+    lengths[-1] = 1000
+    cache, keys, values = filled(lengths, 1, 64, 1024, torch.bfloat16, False, seed=2)
+    q = randn((4097, 2, 64), torch.bfloat16, seed=3).to(DEV)
+    out = FusedPagedDecodeAttention.apply(q, cache, torch.tensor(lengths, dtype=torch.int32, device=DEV), 0.125)
+    some = [0, 1, 2, 4094, 4095, 4096]
+    check_decode(out[some], q[some], [keys[i] for i in some], [values[i] for i in some], [lengths[i] for i in some], 0.125,
+                 0, torch.bfloat16)
+
+
 def test_decode_scores_far_apart():
     """A maximum that keeps rising by more than an exponential can hold, and one key that outweighs the rest."""
     n, d = 500, 64

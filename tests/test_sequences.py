@@ -251,3 +251,16 @@ def test_generate_refuses_what_sampling_and_lists_do_not_take():
     with pytest.raises(RuntimeError, match="ROCm device"):
         model.generate([ids[0]], max_length=5)
     assert model.generate([], max_length=5) == []
+
+
+def test_decode_workspace_fits_every_launch_of_a_call():
+    """A call of more sequences than one launch takes (4096) ends with a smaller launch, which must not want more
+    than the call's workspace; what kind of launch it is goes by the whole call."""
+    need = _lib.load().oslo_attention_paged_decode_workspace_bytes
+    for heads, kv_heads, d in ((1, 1, 64), (2, 1, 128), (8, 8, 256), (34, 2, 64)):
+        for length in (32, 64, 256, 512, 528, 1024, 1040, 4096, 131072):
+            for window in (0, 40, 700):
+                whole = need(4097, heads, kv_heads, d, length, window)
+                assert whole == need(4096, heads, kv_heads, d, length, window)
+                if whole:
+                    assert max(need(n, heads, kv_heads, d, length, window) for n in range(1, 4096, 7)) <= whole
