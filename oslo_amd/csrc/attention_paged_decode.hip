@@ -236,12 +236,14 @@ __device__ __forceinline__ int list_chunks(const PagedDecodeArgs &a, int *first,
 }
 
 // Blocks of a CU the kernel is compiled (and the grid is sized) for. (Four at 128 features: 129 us
-// instead of 96 at 131071 positions; six at 64: 81 instead of 56 at 8 x 16000 positions.)
-constexpr int blocks_per_cu(int D) { return D == 256 ? 2 : D == 128 ? 3 : 4; }
+// instead of 96 at 131071 positions; six at 64: 81 instead of 56 at 8 x 16000 positions. In 8 bits a tile
+// takes half the registers: four at 128 features, 105 us instead of 109 at 128 sequences of 100 to 8191 positions;
+// five spill, and three at 256 do: 325 instead of 191.)
+constexpr int blocks_per_cu(int D, bool e4m3) { return D == 256 ? 2 : D == 128 && !e4m3 ? 3 : 4; }
 
 // MEET: a block per sequence and head slot, whose waves share its tiles and meet in LDS.
 template <typename T, int D, bool E4M3, bool MEET>
-__global__ __launch_bounds__(kBlockThreads, blocks_per_cu(D)) void attention_paged_decode_kernel(const PagedDecodeArgs a) {
+__global__ __launch_bounds__(kBlockThreads, blocks_per_cu(D, E4M3)) void attention_paged_decode_kernel(const PagedDecodeArgs a) {
   using Op = Mfma16<T>;
   using Frag = typename Op::Frag;
   using VL = ValueLayout<D, E4M3>;
@@ -651,7 +653,7 @@ struct DecodeGrid {
 };
 // `sequences` of the `all` of a call.
 inline DecodeGrid decode_grid(int64_t sequences, int64_t all, int64_t kv_heads, int64_t column_groups, int64_t head_dim,
-                              int64_t max_length, int64_t window) {
+                              bool e4m3, int64_t max_length, int64_t window) {
   // (a window may begin anywhere in its first tile)
   const int64_t span = window > 0 && window < max_length ? std::min(window + kTileKeys - 1, max_length) : max_length;
   const int64_t per_sequence = std::max<int64_t>(1, (span + kMinChunk - 1) / kMinChunk);
@@ -665,7 +667,7 @@ inline DecodeGrid decode_grid(int64_t sequences, int64_t all, int64_t kv_heads, 
     return g;
   }
   // (few chunks: a block for each, so that they spread over the CUs)
-  g.blocks = std::min<int64_t>(256 * blocks_per_cu((int)head_dim), sequences * per_sequence * slots);
+  g.blocks = std::min<int64_t>(256 * blocks_per_cu((int)head_dim, e4m3), sequences * per_sequence * slots);
   g.chunks = std::min(sequences * per_sequence,
                       full_chunks(kWavesPerBlock * g.blocks, sequences * slots) / slots + 1 + sequences);
   g.join = per_sequence > 1;
@@ -684,7 +686,8 @@ int launch_paged_decode(PagedDecodeArgs a, int64_t max_length, hipStream_t strea
     part.lengths = a.lengths + s0;
     part.q = static_cast<const T *>(a.q) + s0 * a.q_seq;
     part.out = static_cast<T *>(a.out) + s0 * a.heads * D;
-    const DecodeGrid grid = decode_grid(n, sequences, a.map.kv_heads, a.column_groups, D, max_length, a.window);
+    const DecodeGrid grid = decode_grid(n, sequences, a.map.kv_heads, a.column_groups, D, a.key_scales != nullptr,
+                                        max_length, a.window);
     const int64_t slots = (int64_t)a.map.kv_heads * a.column_groups;
     part.full_chunks = (double)full_chunks(kWavesPerBlock * grid.blocks, n * slots) / (double)slots;
     part.plan = grid.join ? reinterpret_cast<int *>(a.partial) : nullptr;
@@ -727,9 +730,13 @@ extern "C" size_t oslo_attention_paged_decode_workspace_bytes(int64_t sequences,
   if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_length <= 0 || heads % kv_heads) return 0;
   const int64_t groups = (heads / kv_heads + kColumns - 1) / kColumns;
   const int64_t n = std::min<int64_t>(sequences, kMaxSequences); // (of one launch)
-  const DecodeGrid g = decode_grid(n, sequences, kv_heads, groups, head_dim, max_length, window);
-  if (!g.join) return 0;
-  return ((size_t)plan_ints(n) + (size_t)g.chunks * (size_t)heads * (size_t)(head_dim + 4)) * sizeof(float);
+  int64_t chunks = 0; // (of either kind of cache)
+  for (const bool e4m3 : {false, true}) {
+    const DecodeGrid g = decode_grid(n, sequences, kv_heads, groups, head_dim, e4m3, max_length, window);
+    if (!g.join) return 0;
+    chunks = std::max(chunks, g.chunks);
+  }
+  return ((size_t)plan_ints(n) + (size_t)chunks * (size_t)heads * (size_t)(head_dim + 4)) * sizeof(float);
 }
 
 extern "C" int oslo_attention_paged_decode_fwd(void *out, const void *q, const void *key_pages,
@@ -766,7 +773,7 @@ extern "C" int oslo_attention_paged_decode_fwd(void *out, const void *q, const v
   a.group = (int)(heads / kv_heads);
   a.column_groups = (a.group + kColumns - 1) / kColumns;
   if (!workspace && decode_grid(std::min<int64_t>(sequences, kMaxSequences), sequences, kv_heads, a.column_groups, head_dim,
-                                max_length, window).join)
+                                key_scales != nullptr, max_length, window).join)
     return fail(OSLO_E_BAD_ARG, "%s: null workspace", name);
   if (!aligned16(workspace)) return fail(OSLO_E_UNSUPPORTED, "%s: the workspace must be 16-byte aligned", name);
   a.out = out, a.q = q, a.q_seq = strides[0], a.q_head = strides[1];
