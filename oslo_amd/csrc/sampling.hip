@@ -115,6 +115,10 @@ __device__ __forceinline__ u64 wave_scan_u64(u64 v) {
   v += dpp_u64<0x143, 0xc>(v);
   return v;
 }
+__device__ __forceinline__ u64 lane_u64(u64 v, int lane) { // (of a lane that is the same for all)
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
 // Sum over the wave, for every lane: rows of 16 on the vector ALU, the four rows by lane reads.
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
   v += dpp_u64<0xB1>(v);
@@ -567,13 +571,11 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     r.missing = target;
     return r;
   };
-  // In the chunk of 64 pieces from `piece` on, which the calling wave takes and before
-  // which the running weight is `before`: f(index, logit) where it exceeds `target`, by one lane.
-  auto inside_chunk = [&](int piece, u64 before, auto &&weight, u64 target, auto &&f) __attribute__((always_inline)) {
-    piece += lane;
-    const V v = load(piece);
-    u64 w[kVec], sum = 0;
-    weight(v, first_in(piece), w);
+  // Of a chunk of 64 pieces, before which the running weight is `before`, the lane has the piece v with the
+  // weights w: f(index, logit) where the running weight exceeds `target`, by one lane.
+  auto inside_chunk = [&](const V &v, const u64 (&w)[kVec], int piece, u64 before, u64 target, auto &&f)
+                          __attribute__((always_inline)) {
+    u64 sum = 0;
 #pragma unroll
     for (int e = 0; e < kVec; ++e) sum += w[e];
     u64 at = before + wave_scan_u64(sum) - sum;
@@ -596,11 +598,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     });
     __syncthreads();
     const Found f = find_bin(lds, scan_bins<kThreads>(lds), ties);
-    if (wave == 0)
-      inside_chunk(f.at * kWave, f.before, [&](const V &v, int first, u64 (&w)[kVec]) __attribute__((always_inline)) {
+    if (wave == 0) {
+      const int piece = f.at * kWave + lane;
+      const V v = load(piece);
+      u64 w[kVec];
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) w[e] = is_tie(static_cast<float>(v[e]), first + e);
-      }, ties - 1, [&](int index, float) __attribute__((always_inline)) { lds.found_at = index; });
+      for (int e = 0; e < kVec; ++e) w[e] = is_tie(static_cast<float>(v[e]), first_in(piece) + e);
+      inside_chunk(v, w, piece, f.before, ties - 1,
+                   [&](int index, float) __attribute__((always_inline)) { lds.found_at = index; });
+    }
     __syncthreads();
     const int index = lds.found_at;
     __syncthreads();
@@ -954,43 +960,48 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
   __syncthreads();
   // The draw: the wave in whose run of the row the running mass passes the target, its
   // chunk (every wave sums some), and the logit in it.
-  u64 total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) total += lds.wave_kept[w];
+  const u64 waves_upto = wave_scan_u64(lane < kWaves ? lds.wave_kept[lane] : 0);
+  const u64 total = lane_u64(waves_upto, kWaves - 1);
   const u64 target = drawn_of(total);
-  u64 before = 0;
-  int from = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const u64 upto = before + lds.wave_kept[w];
-    if (upto <= target && from == w) before = upto, from = w + 1;
-  }
-  const int first_chunk = from * chunks; // (from < kWaves: the target is below the total)
+  const int from = __popcll(__ballot(lane < kWaves && waves_upto <= target)); // (< kWaves: the target is below the total)
+  u64 before = from > 0 ? lane_u64(waves_upto, from - 1) : 0;
+  const int first_chunk = from * chunks;
   if (wave == kWaves - 1) { // (the wave that has the fewest of the chunks below)
     const double log_total = log_of(total);
     if (lane == 0) lds.log_total = log_total;
   }
+  V v{};
+  u64 w[kVec];
+  auto weigh = [&](int c) __attribute__((always_inline)) {
+    const int piece = (first_chunk + c) * kWave + lane;
+    v = load(piece);
+    kept_of(v, first_in(piece), w);
+  };
+  int weighed = -1; // the chunk that v and w are of
 #pragma unroll 1
   for (int c = wave; c < chunks; c += kWaves) {
-    const int piece = (first_chunk + c) * kWave + lane;
-    const V v = load(piece);
-    u64 w[kVec], sum = 0;
-    kept_of(v, first_in(piece), w);
+    weigh(c);
+    u64 sum = 0;
 #pragma unroll
     for (int e = 0; e < kVec; ++e) sum += w[e];
     sum = wave_sum_u64(sum);
     if (lane == 0) lds.list[c] = sum; // (the list is read no more)
+    weighed = c;
   }
   __syncthreads();
   int c = 0;
-#pragma unroll 8
-  for (int i = 0; i < chunks - 1; ++i) {
-    const u64 upto = before + lds.list[i];
-    if (upto <= target && c == i) before = upto, c = i + 1;
+#pragma unroll 1
+  while (true) { // 64 chunks at a time: those that end before the target
+    const u64 upto = before + wave_scan_u64(c + lane < chunks ? lds.list[c + lane] : 0);
+    const int passed = __popcll(__ballot(c + lane < chunks - 1 && upto <= target));
+    if (passed > 0) before = lane_u64(upto, passed - 1);
+    c += passed;
+    if (passed < kWave) break;
   }
-  if (wave == c % kWaves)
-    inside_chunk((first_chunk + c) * kWave, before, kept_of, target, [&](int index, float x)
-                     __attribute__((always_inline)) { finish(index, x, lds.log_total); });
+  if (wave != c % kWaves) return;
+  if (c != weighed) weigh(c);
+  inside_chunk(v, w, (first_chunk + c) * kWave + lane, before, target, [&](int index, float x)
+                   __attribute__((always_inline)) { finish(index, x, lds.log_total); });
 }
 
 // Logits a row may have: its chunks have to fit the bins, and the list.
