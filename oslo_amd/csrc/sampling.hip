@@ -169,21 +169,16 @@ struct BinScan {
 template <int kThreads>
 __device__ __forceinline__ BinScan<kThreads> scan_values(SampleLds &lds, BinScan<kThreads> s) {
   constexpr int kBinsEach = s.kEach, kWaves = kThreads / kWave;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   s.mine = 0;
 #pragma unroll
   for (int i = 0; i < kBinsEach; ++i) s.mine += s.v[i];
   const u64 upto = wave_scan_u64(s.mine);
   if (lane == kWave - 1) lds.wave_sums[wave] = upto;
   __syncthreads();
-  s.before = upto - s.mine;
-  s.total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const u64 v = lds.wave_sums[w];
-    if (w < wave) s.before += v;
-    s.total += v;
-  }
+  const u64 waves = wave_scan_u64(lane < kWaves ? lds.wave_sums[lane] : 0);
+  s.before = upto - s.mine + (wave > 0 ? lane_u64(waves, wave - 1) : 0);
+  s.total = lane_u64(waves, kWaves - 1);
   return s;
 }
 // The bins must be complete (a barrier has passed).
@@ -895,9 +890,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     if (lane == 0) lds.wave_kept[wave] = wave_kept, lds.wave_all[wave] = wave_all;
     __syncthreads();
     if (!window) break;
-    u64 total = 0, above = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) total += lds.wave_all[w], above += lds.wave_kept[w];
+    const u64 total = wave_sum_u64(lane < kWaves ? lds.wave_all[lane] : 0);
+    const u64 above = wave_sum_u64(lane < kWaves ? lds.wave_kept[lane] : 0);
     const u64 target = share_of(total);
     const int n = lds.listed;
     if (by_floor && above <= target) break;
