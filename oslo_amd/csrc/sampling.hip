@@ -24,7 +24,7 @@
 // is read again, ahead of its use), each wave a run of it. Such a row is read in 5 to 8 us; what
 // costs the time then is arithmetic, one operation in 64 bits after another, and
 // barriers (one row of 1024 threads, thousands of cycles: reading 10, the count below 12, its
-// border 4, the exact pass 30, the border in the window 5 to 7, the draw 11):
+// border 3.5, the exact pass 30, the border in the window 5 to 7, the draw 5.5):
 //  - top-k goes first: a histogram of the threads' own maxima gives a bound that
 //    at least k logits reach and few exceed. They go into a list in LDS, which is all
 //    the rest looks at; up to 512 of them are ranked by counting, without a sort.
@@ -40,7 +40,7 @@
 //    chunk, which all waves sum together, and looks inside that.
 // Windows too full for the list (equal logits by the thousand) are searched by
 // histograms over the bits of the logits. Measured, us a call: one row of 50257 fp32 logits, top-k 50 and
-// top-p, 12.6; 256 rows in bf16, settings of their own, 39; 1000 rows in fp32, top-p 0.92, 120 to 130.
+// top-p, 12.3; 256 rows in bf16, settings of their own, 36; 1000 rows in fp32, top-p 0.92, 118 to 127.
 
 #include "common.hpp"
 
