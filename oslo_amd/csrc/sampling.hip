@@ -607,11 +607,12 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
     __syncthreads();
     return index;
   };
-  // The front now ends at b.key, of whose logits the first ceil(b.missing / each) are in.
+  // The front now ends at b.key, of whose logits the first ceil(b.missing / each) are in. (All that were counted:
+  // those up to the front's old end, where that lies among them.)
   auto set_cut = [&](const Border &b, u64 each) __attribute__((always_inline)) {
     const u64 ties = (b.missing + each - 1) / each;
     const float x = key_value(b.key);
-    const int index = ties < b.value / each ? index_of_tie(x, ties) : vocab;
+    const int index = ties < b.value / each ? index_of_tie(x, ties) : cutting && x == cut ? cut_index : vocab;
     cut = x;
     cut_index = index;
     cutting = true;

@@ -216,3 +216,22 @@ def test_logits_as_far_apart_as_the_type_allows(vocab):
     for kw in (dict(), dict(top_k=5), dict(top_k=300), dict(top_k=900, top_p=0.7), dict(top_p=0.9), dict(min_p=0.2),
                dict(top_k=50, temperature=1.0e37), dict(top_p=0.5, temperature=1.0e-37)):
         check(logits, u, **kw)
+
+
+@pytest.mark.parametrize("rows", [4, 260], ids=["few-rows", "many-rows"])
+@pytest.mark.parametrize("vocab", [8000, 50257])
+def test_top_p_does_not_bring_back_what_top_k_left_out(vocab, rows):
+    """More equal logits at top-k's border than the list holds (2048), of which top-p keeps all that top-k
+    kept: whole masses of 1, so the plain sums are exact."""
+    u = (torch.arange(rows, device=DEV, dtype=torch.float32) + 0.9) / rows
+    flat = torch.full((rows, vocab), 0.75, device=DEV)
+    some = flat.clone()
+    some[:, 5::1000] = 1.5          # a few above the equal ones
+    steps = flat.clone()
+    steps[:, ::2] = 0.75 - 2.0 ** -20   # two values within a step of the count
+    for logits in (flat, some, steps):
+        for k in (2049, 3000, 4000):
+            for p in (0.5, 0.9999, 0.99999):
+                tokens = check(logits, u, top_k=k, top_p=p)
+                if logits is flat and p > 0.9:
+                    assert torch.equal(tokens, torch.floor(u.double() * k).long())
