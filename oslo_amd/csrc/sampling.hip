@@ -1048,7 +1048,10 @@ extern "C" int oslo_sample(int64_t *tokens, float *logprobs, const void *logits,
   if (!tokens || !logits || !uniforms) return fail(OSLO_E_BAD_ARG, "oslo_sample: null pointer");
   SampleArgs a;
   a.tokens = tokens, a.logprobs = logprobs, a.logits = logits, a.row_stride = row_stride, a.uniforms = uniforms;
-  a.temperature = {temperatures, temperature};
+  // (Logits that differ do so by 2^-149 at least: from here down all but the largest have mass 0, and the reciprocal
+  // would leave the range of 64 bits. Temperatures of a row's own have 32 bits and cannot come near.)
+  constexpr double kLeastTemperature = 1.0e-300;
+  a.temperature = {temperatures, temperature > 0.0 && temperature < kLeastTemperature ? kLeastTemperature : temperature};
   a.top_k = {top_ks, (double)top_k};
   a.top_p = {top_ps, top_p};
   a.min_p = {min_ps, min_p};

@@ -235,3 +235,19 @@ def test_top_p_does_not_bring_back_what_top_k_left_out(vocab, rows):
                 tokens = check(logits, u, top_k=k, top_p=p)
                 if logits is flat and p > 0.9:
                     assert torch.equal(tokens, torch.floor(u.double() * k).long())
+
+
+def test_temperatures_next_to_zero():
+    """Positive ones, down to the smallest number there is: the largest logits share the draw (0 takes the first)."""
+    logits = torch.tensor([[1.0, 3.0, 2.0, 3.0, -1.0, 3.0], [0.0, -2.0 ** -149, 2.0 ** -149, 0.0, 0.0, 0.0],
+                           [-3.0e38, 3.0e38, 3.0e38, 0.0, float("-inf"), float("nan")]], device=DEV)
+    for rows in (3, 300):
+        x = logits.repeat(rows // 3, 1)
+        u = torch.rand((rows,), generator=torch.Generator().manual_seed(3)).to(DEV)
+        for t in (5e-324, 1e-310, 1e-306, 7e-306, 1e-300):
+            for kw in (dict(), dict(top_k=2), dict(top_p=0.5), dict(min_p=0.5), dict(top_k=4, top_p=0.4, min_p=1.0)):
+                tokens = check(x, u, temperature=t, **kw)
+                assert tokens[1::3].eq(2).all()
+        each = torch.full((rows,), 2.0 ** -149, device=DEV)
+        check(x, u, temperature=each, top_p=0.5)
+        check(x, u, temperature=2.0 ** -149, top_p=0.5)
