@@ -189,8 +189,9 @@ class PackedLayer(SequenceLayer):
 class PagedState(object):
     """The layers' paged caches while one token per sequence is decoded at a
     time, under one table, with pages for ``capacity`` positions of each sequence.
-    ``lengths`` (int32 [sequences] on the device) counts the positions written,
-    which is also the position of the token being fed: nothing in a step depends
+    ``lengths`` (int32 [sequences] on the device) is the position of the token being
+    fed: the number of positions written, or the last position of a sequence that is
+    full, which its next tokens overwrite. Nothing in a step depends
     on the host, so a step can be captured into a graph and replayed."""
 
     def __init__(self, lengths, capacity, layers, kv_heads, head_dim, dtype, device, page_size=64, quantized=False):
@@ -200,7 +201,8 @@ class PagedState(object):
         each = -(-self.capacity // page_size)
         num_pages = len(lengths) * each
         self.table = torch.arange(num_pages, dtype=torch.int32, device=device).view(len(lengths), each)
-        self.lengths = torch.tensor([int(n) for n in lengths], dtype=torch.int32, device=device)
+        # (a sequence that is full feeds its next token to its last position, like one that gets there by steps)
+        self.lengths = torch.tensor([min(int(n), self.capacity - 1) for n in lengths], dtype=torch.int32, device=device)
         self.visible = self.lengths + 1
         self.rows = torch.arange(len(lengths), dtype=torch.int32, device=device)
         self.step_values = {}  # what layers share within one step
@@ -219,8 +221,7 @@ class PagedState(object):
         return [PagedLayer(self, cache) for cache in self.caches]
 
     def end_step(self):
-        """The tokens are in the cache. A sequence that is full stays at its last
-        position, which its next tokens overwrite."""
+        """The tokens are in the cache."""
         self.lengths.add_(1).clamp_(max=self.capacity - 1)
 
 

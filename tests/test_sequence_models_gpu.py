@@ -288,3 +288,27 @@ def test_devices_of_a_state_and_a_model_must_agree():
     state = PagedState([0, 0], 8, 1, 2, 64, torch.bfloat16, DEV)
     with pytest.raises(RuntimeError, match="cache"), torch.no_grad():
         model(torch.zeros((1, 2), dtype=torch.long, device=DEV), past_key_values=state.begin_step())
+
+
+@pytest.mark.parametrize("family", FAMILIES)
+def test_a_prompt_that_fills_the_cache_is_followed_by_steps(family):
+    """The model's last position, and the cache's: the next tokens overwrite it, as they do once a sequence has grown
+    to be full."""
+    model, _ = make(family)
+    prompts = [tokens(n, 70 + i).to(DEV) for i, n in enumerate([POSITIONS, 5])]
+    feed = torch.stack([tokens(3, 80 + i) for i in range(2)]).to(DEV)
+    rows = []
+    with torch.no_grad():
+        for first in (POSITIONS, POSITIONS - 1):  # (the position the first step writes, either way)
+            state = PagedState([first, 5], POSITIONS, len(model.transformer.h), 2, 128 if family == "gptj" else 64,
+                               torch.float16, DEV)
+            packed = PackedSequences([len(p) for p in prompts], DEV)
+            model.transformer(torch.cat(prompts)[None], None, state.prompt_layers(packed))
+            rows.append([])
+            for step in range(3):
+                logits = model(feed[None, :, step], past_key_values=state.begin_step())["logits"][0]
+                state.end_step()
+                rows[-1].append(logits.clone())
+        assert state.lengths.tolist() == [POSITIONS - 1, 8]
+    for a, b in zip(*rows):
+        assert a.isfinite().all() and torch.equal(a, b)

@@ -210,6 +210,19 @@ def test_paged_state_gives_every_sequence_its_own_pages_and_stops_at_the_last_po
             PagedState(**bad, layers=1, kv_heads=1, head_dim=64, dtype=torch.float16, device="cpu")
 
 
+def test_a_sequence_that_is_full_from_the_start_stays_at_its_last_position():
+    """Prompts of as many tokens as there are positions: the fed token's position, and what it sees, stay inside."""
+    from oslo_amd.modeling_gptj import rotary_for_step
+    state = PagedState([4, 2, 4], 4, 1, 1, 64, torch.float16, "cpu", page_size=16)
+    for _ in range(2):
+        layer = state.begin_step()[0]
+        assert layer.positions.tolist()[::2] == [3, 3] and int(state.visible.max()) <= state.capacity
+        sin, cos, offset = rotary_for_step(layer, 64, 3, torch.device("cpu"))
+        assert sin.shape == cos.shape == (3, 32) and offset == 0
+        state.end_step()
+    assert state.lengths.tolist() == [3, 3, 3]
+
+
 def test_models_refuse_what_sequences_do_not_take():
     model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
     row, packed = torch.zeros((1, 6), dtype=torch.long), PackedSequences([2, 4], "cpu")
