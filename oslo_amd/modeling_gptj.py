@@ -57,21 +57,43 @@ class GPTJConfig:
 
 
 _rotary_table_cache = {}
+_captured_rotary_tables = {}  # those a captured graph reads, which has to find them for as long as it lives
+
+
+def _capturing(device):
+    return torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing()
 
 
 def rotary_tables(dim, seq_len, device):
     """sin and cos of position * 10000^(-2i/dim), each [seq_len, dim/2], fp32.
-    Every layer asks for the same tables, so the last few are kept."""
+    Every layer asks for the same tables, so the last few are kept; those a graph
+    is captured with stay, and those made inside a capture, which only its
+    replays fill, are not handed to anybody else."""
     key = (int(dim), int(seq_len), str(device))
     hit = _rotary_table_cache.get(key)
     if hit is not None:
+        if _capturing(device):
+            _captured_rotary_tables[key] = hit
         return hit
     inv_freq = 1.0 / (10000 ** (torch.arange(0, dim, 2, device=device, dtype=torch.float32) / dim))
     angles = torch.arange(seq_len, device=device, dtype=torch.float32)[:, None] * inv_freq[None, :]
     tables = (torch.sin(angles), torch.cos(angles))
+    if _capturing(device):
+        return tables
     if len(_rotary_table_cache) >= 8:
         _rotary_table_cache.pop(next(iter(_rotary_table_cache)))
     _rotary_table_cache[key] = tables
+    return tables
+
+
+def _tables_of(kept, dim, positions, device):
+    """The tables of a decode state or of packed sequences, which keep them (in ``kept``): a graph captured over
+    them goes on reading the tables it was captured with."""
+    tables = kept.get((dim, positions))
+    if tables is None:
+        tables = rotary_tables(dim, positions, device)
+        if not _capturing(device):
+            kept[(dim, positions)] = tables
     return tables
 
 
@@ -83,7 +105,7 @@ def rotary_for_step(layer_past, dim, seq_len, device):
     if isinstance(layer_past, SequenceLayer):
         rows = layer_past.shared.get(("rotary", dim, seq_len))
         if rows is None:  # the first layer of a forward gathers them, the others reuse them
-            sin, cos = rotary_tables(dim, max(layer_past.max_position, 1), device)
+            sin, cos = _tables_of(layer_past.kept, dim, max(layer_past.max_position, 1), device)
             at = layer_past.row_positions(seq_len)
             rows = layer_past.shared[("rotary", dim, seq_len)] = (sin.index_select(0, at), cos.index_select(0, at))
         return rows[0], rows[1], 0
@@ -91,7 +113,7 @@ def rotary_for_step(layer_past, dim, seq_len, device):
         state = layer_past.state
         row = state.step_values.get(("rotary", dim))
         if row is None:  # the first layer of a step gathers the row, the others reuse it
-            sin, cos = rotary_tables(dim, state.capacity, device)
+            sin, cos = _tables_of(state.kept, dim, state.capacity, device)
             row = state.step_values[("rotary", dim)] = (sin.index_select(0, state.pos), cos.index_select(0, state.pos))
         return row[0], row[1], 0
     offset = 0 if layer_past is None else layer_past[0].shape[-2]

@@ -108,6 +108,7 @@ class DecodeState(object):
         self.slots = torch.arange(self.capacity, device=device)
         self._hidden = {}  # window (None: all earlier keys) -> bool [1,1,1,capacity], True = hidden
         self.step_values = {}  # what layers share within one step (the rotary table row of ``pos``)
+        self.kept = {}  # what outlives a step: the rotary tables, which a captured step reads
 
     def begin_step(self):
         """Recomputes the masks from ``pos``; called once per step, before the

@@ -43,6 +43,7 @@ class PackedSequences(object):
         self.blocks = torch.from_numpy(np.stack([entries[o] for o in order])).to(device)
         self._queries = queries[order[1]]  # of the blocks with most queries first: how many are left
         self._shared = {}
+        self.kept = {}  # what the models look up for these sequences (rotary tables), for as long as they live
         self._positions = self._sequence = None
 
     @property
@@ -155,9 +156,9 @@ class SequenceLayer(object):
     [T, H, D], key and value [T, Hkv, D] and returns [T, H, D]; ``positions``
     (int32 on the device) are the tokens' positions in their sequences, all
     below ``max_position``; ``shared`` holds what the layers of one forward
-    work out once."""
+    work out once, ``kept`` what stays for the next one."""
 
-    positions = max_position = shared = None
+    positions = max_position = shared = kept = None
 
     def row_positions(self, tokens):
         """``positions`` for a row of ``tokens``: 0 behind the last sequence (such
@@ -176,7 +177,7 @@ class PackedLayer(SequenceLayer):
     with ``cache`` their keys and values also go into that layer's ``PagedKV``."""
 
     def __init__(self, packed, cache, shared):
-        self.packed, self.cache, self.shared = packed, cache, shared
+        self.packed, self.cache, self.shared, self.kept = packed, cache, shared, packed.kept
         self.positions, self.max_position = packed.positions, packed.max_length
 
     def attend(self, query, key, value, scale, window=None):
@@ -206,6 +207,7 @@ class PagedState(object):
         self.visible = self.lengths + 1
         self.rows = torch.arange(len(lengths), dtype=torch.int32, device=device)
         self.step_values = {}  # what layers share within one step
+        self.kept = {}  # what outlives a step: the rotary tables, which a captured step reads
         self.caches = [PagedKV.allocate(self.table, num_pages, kv_heads, page_size, head_dim, dtype, device, quantized)
                        for _ in range(layers)]
 
@@ -229,7 +231,7 @@ class PagedLayer(SequenceLayer):
     """One new token per sequence over a layer's paged cache."""
 
     def __init__(self, state, cache):
-        self.state, self.cache, self.shared = state, cache, state.step_values
+        self.state, self.cache, self.shared, self.kept = state, cache, state.step_values, state.kept
         self.positions, self.max_position = state.lengths, state.capacity
 
     def attend(self, query, key, value, scale, window=None):

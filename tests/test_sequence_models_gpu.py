@@ -312,3 +312,74 @@ def test_a_prompt_that_fills_the_cache_is_followed_by_steps(family):
         assert state.lengths.tolist() == [POSITIONS - 1, 8]
     for a, b in zip(*rows):
         assert a.isfinite().all() and torch.equal(a, b)
+
+
+def forget_rotary_tables():
+    """Other lengths are asked for until the last tables have gone, and memory of their size is written over."""
+    from oslo_amd.modeling_gptj import rotary_tables
+    for n in range(700, 720):
+        rotary_tables(32, n, torch.device(DEV))
+    return [torch.full((n, 16), float("nan"), device=DEV) for n in range(8, 400, 8) for _ in range(4)]
+
+
+def test_captured_graphs_keep_their_rotary_tables():
+    """A captured decoding step over paged and static caches and a captured forward, replayed after the tables of many
+    other lengths have been made."""
+    model, _ = make("gptj")
+    ids = tokens(60, 5)[None].to(DEV)
+    with torch.no_grad():
+        state = PagedState([9, 30], 40, len(model.transformer.h), 2, 128, torch.float16, DEV)
+        packed = PackedSequences([9, 30], DEV)
+        feed = torch.stack([tokens(2, i) for i in (1, 2)]).to(DEV)
+        forget_rotary_tables()
+
+        def step():
+            return model(feed[:1], past_key_values=state.begin_step())["logits"]
+
+        def row():
+            return model(ids[:, :39], packed=packed)["logits"]
+
+        def dense():
+            return model(ids[:, :45])["logits"]
+        model.transformer(ids[:, :39], None, state.prompt_layers(packed))
+        for run in (step, row, dense):
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                run()
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = run()
+            junk = forget_rotary_tables()
+            for _ in range(3):
+                want = run().clone()
+                forget_rotary_tables()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert want.isfinite().all() and torch.equal(out, want)
+            del junk
+        # a graph that generate() keeps
+        first = model.generate(ids[:, :20], max_length=50, static_cache=True, graph=True)
+        junk = forget_rotary_tables()
+        assert torch.equal(model.generate(ids[:, :20], max_length=50, static_cache=True, graph=True), first)
+        del junk
+
+
+def test_rotary_tables_made_inside_a_capture_are_not_handed_on():
+    """Without a warm-up the tables are filled by the replays alone."""
+    from oslo_amd.modeling_gptj import rotary_tables
+    device = torch.device(DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made = rotary_tables(32, 333, device)
+    other = rotary_tables(32, 333, device)
+    want = torch.sin(torch.arange(333.0)[:, None] / 10000 ** (torch.arange(0, 32, 2.0) / 32))
+    assert (other[0].cpu() - want).abs().max() < 1e-4
+    for _ in range(3):
+        made[0].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(made[0], other[0]) and torch.equal(made[1], other[1])

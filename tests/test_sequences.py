@@ -223,6 +223,33 @@ def test_a_sequence_that_is_full_from_the_start_stays_at_its_last_position():
     assert state.lengths.tolist() == [3, 3, 3]
 
 
+def test_rotary_tables_live_as_long_as_what_reads_them():
+    """A captured step goes on reading its tables, whatever other lengths are asked for in between."""
+    import weakref
+
+    from oslo_amd import DecodeState, StaticKV
+    from oslo_amd import modeling_gptj as gptj
+    state = PagedState([4, 2], 37, 1, 1, 64, torch.float16, "cpu", page_size=16)
+    packed = PackedSequences([29, 3], "cpu")
+    static = DecodeState(41, "cpu", torch.float16)
+    layers = [(state.begin_step()[0], 2), (sequence_layers(packed, 1)[0], 32),
+              (StaticKV(static, *(torch.zeros((1, 1, 41, 64)) for _ in range(2))), 1)]
+    device = torch.device("cpu")
+    tables = []
+    for (layer, n), positions in zip(layers, (37, 29, 41)):
+        gptj.rotary_for_step(layer, 32, n, device)
+        tables.append([weakref.ref(t) for t in gptj.rotary_tables(32, positions, device)])
+    del layer, layers
+    for n in range(50, 70):
+        gptj.rotary_tables(32, n, device)
+    for holder, refs in zip((state, packed, static), tables):
+        assert all(r() is not None for r in refs)
+    del state, packed, static, holder
+    import gc
+    gc.collect()
+    assert all(r() is None for refs in tables for r in refs)
+
+
 def test_models_refuse_what_sequences_do_not_take():
     model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
     row, packed = torch.zeros((1, 6), dtype=torch.long), PackedSequences([2, 4], "cpu")
