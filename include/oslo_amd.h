@@ -653,7 +653,8 @@ int oslo_attention_packed_bwd(void *dq, void *dk, void *dv, const void *dout,
  * they are OCP e4m3: a vector x of head_dim features is kept as
  * q = round_to_nearest_even_e4m3(x * 2^-e) and the byte e + 127, e the least
  * integer >= -126 with max|x| <= 448 * 2^e over the finite features (0 if they
- * are all 0); infinities and NaN are kept as NaN.
+ * are all 0); infinities and NaN are kept as NaN, and magnitudes of an fp16 vector above
+ * 61440 as 61440 (the next number of this storage, 65536, is beyond fp16).
  *
  * write: token t of key, value ([tokens, kv_heads, head_dim] of `dtype`;
  * strides[4] = head and token strides of key, then of value, in elements,
@@ -702,8 +703,10 @@ size_t oslo_attention_paged_decode_workspace_bytes(int64_t sequences,
  * replayed while they grow. A sequence of length 0 (or less) gives zeros; one that
  * is longer than its table, or that would read a page number outside the pool,
  * gives NaN and reads nothing out of bounds. Positions outside the visible ones
- * are not looked at, whatever they hold. Products are of 16-bit values (an 8-bit
- * cache's are exact in either type), sums and the softmax fp32, probabilities
+ * are not looked at, whatever they hold. Products are of 16-bit values (those of an
+ * 8-bit cache are exact, but for values times their scale that fp16 has no normal number for:
+ * below 2^-14 they are rounded to multiples of 2^-24, above 65504, in a cache written in
+ * bf16, infinite), sums and the softmax fp32, probabilities
  * rounded to 16 bits before they multiply v, the result rounded once. The joining
  * order is fixed: same bits from run to run. workspace:
  * oslo_attention_paged_decode_workspace_bytes bytes, 16-byte aligned, contents

@@ -11,8 +11,10 @@
 // integer with max|x| <= 448 * 2^e (448 is e4m3's largest number). A power of two
 // costs a floating-point format no precision (only the exponents move) and makes
 // both directions exact but for the one rounding to e4m3: x * 2^-e and q * 2^e are
-// exact in fp32, and q * 2^e is a bf16 or fp16 number wherever it is in range, so
-// the matrix cores read the values themselves, not roundings of them.
+// exact in fp32, and q * 2^e is a bf16 or fp16 number wherever it is in the type's
+// normal range, so the matrix cores read the values themselves, not roundings of
+// them. In fp16 products below 2^-14 may be rounded, to multiples of 2^-24; those above 65504,
+// which only a cache written in bf16 can hold, are infinite.
 #pragma once
 
 #include "common.hpp"
@@ -40,8 +42,8 @@ __device__ __forceinline__ float exponent_to_scale(int biased) { // 2^(biased - 
   return __builtin_bit_cast(float, (uint32_t)biased << 23);
 }
 
-// Two e4m3 numbers (the low or the high half of a word) times 2^e, as T. The
-// products are exact in bf16, and in fp16 wherever they are in its range.
+// Two e4m3 numbers (the low or the high half of a word) times 2^e, as T (exact in the
+// type's normal range).
 template <typename T>
 using Pair = typename VecOf<T, 2>::type;
 template <bool HIGH>

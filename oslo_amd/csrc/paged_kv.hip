@@ -1,7 +1,8 @@
 // Keys and values of new tokens into the paged cache, and back out of it: one
 // pass over the tokens' vectors each way, in 16 bits (a copy) or 8 bits
 // (e4m3 with a power-of-two scale per token and head, paged.hpp):
-//   write: e = least integer with max|x| <= 448 * 2^e;  q = round_to_e4m3(x * 2^-e)
+//   write: e = least integer with max|x| <= 448 * 2^e;  q = round_to_e4m3(x * 2^-e), x in fp16
+//          at most 61440 so that it can be read back
 //   read:  x = q * 2^e
 // The vector of one token and head is held by D / 8 lanes, 16 bytes each, so
 // its largest magnitude is a reduction inside those lanes and it is read once.
@@ -50,6 +51,11 @@ __device__ __forceinline__ float max_over_lanes(float v) {
   return v;
 }
 
+// The largest number of the 8-bit storage that fp16 has: 240 * 2^8 (the next, 256 * 2^8, is
+// infinity there). Larger ones of an fp16 vector, up to 65504, are taken to it: 6.2 % off, where
+// the rounding to e4m3 may be off by 2^-4. Vectors with smaller scales hold nothing so large.
+constexpr float kMostF16 = 61440.0f;
+
 template <typename T, int D>
 __device__ __forceinline__ void store_e4m3(unsigned char *pages, unsigned char *scales, int64_t slot, int part,
                                            const RawVec<T, 8> &raw) {
@@ -63,7 +69,11 @@ __device__ __forceinline__ void store_e4m3(unsigned char *pages, unsigned char *
   const float inverse = exponent_to_scale(127 - e);
   // (infinities and NaN have no scaled value: they are kept as NaN)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __builtin_isfinite(x[i]) ? x[i] * inverse : __builtin_nanf("");
+  for (int i = 0; i < 8; ++i) {
+    float y = x[i];
+    if constexpr (std::is_same<T, f16>::value) y = __builtin_amdgcn_fmed3f(y, -kMostF16, kMostF16);
+    x[i] = __builtin_isfinite(x[i]) ? y * inverse : __builtin_nanf("");
+  }
   u32x2 w;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {

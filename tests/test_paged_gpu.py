@@ -385,3 +385,50 @@ def test_refused_calls():
     assert FusedPagedDecodeAttention.is_available(q, cache)
     assert not FusedPagedDecodeAttention.is_available(q.half(), cache)
     assert not FusedPagedDecodeAttention.is_available(q, cache, True, 0.1)
+
+
+def test_eight_bit_values_at_the_ends_of_fp16():
+    """Every finite fp16 number comes back finite: at the top the nearest number of the storage that fp16 has, 240 * 2^8;
+    below the normal numbers the product rounded to fp16."""
+    d, rows = 64, []
+
+    def row(*values):
+        rows.append(torch.tensor(list(values) + [0.0] * (d - len(values)), dtype=torch.float64))
+    row(65504.0, -65504.0, 63520.0, 63488.0, 63456.0, -61472.0, 61440.0, 59000.0, 1.0, 0.25)
+    row(-61472.0, 3.0)
+    row(57376.0, 100.0)
+    row(57344.0, -57344.0, 100.0)
+    row(60000.0, float("inf"), float("nan"), -65504.0)
+    row(2.0 ** -24, -2.0 ** -23, 3 * 2.0 ** -24)
+    row(2.0 ** -14, 2.0 ** -15, 2.0 ** -24, 1023 * 2.0 ** -24)
+    x = torch.stack(rows).to(torch.float16)[:, None, :].to(DEV)
+    assert x[0, 0, 0] == 65504.0
+    cache = poisoned([len(rows)], 1, d, 16, torch.float16, True)
+    seq, pos = tokens_of([len(rows)])
+    FusedPagedKV.write(cache, x, x.flip(0), seq, pos)
+    key, value = FusedPagedKV.read(cache, seq, pos, torch.float16)
+    for got, src in ((key, x), (value, x.flip(0))):
+        want = stored(src.clamp(-61440.0, 61440.0).where(src.isfinite(), src)).to(torch.float16)
+        assert torch.equal(got.cpu().nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(got.isnan().cpu(), want.isnan())
+        assert torch.equal(got.isfinite(), src.isfinite())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_large_values_of_keys_that_do_not_count(d):
+    """A value at the end of fp16 under a probability that rounds to zero changes nothing."""
+    n, dtype = 70, torch.float16
+    cache = poisoned([n], 2, d, 16, dtype, True)
+    seq, pos = tokens_of([n])
+    k, v = (randn((n, 2, d), dtype, seed=s).to(DEV) for s in (1, 2))
+    q = randn((1, 4, d), dtype, seed=3).to(DEV)
+    q[..., 0] = 1.0
+    k[..., 0] = 0.0
+    k[33, :, 0] = -1000.0
+    v[33, :, :] = 65504.0
+    v[33, :, 1::2] = -65504.0
+    FusedPagedKV.write(cache, k, v, seq, pos)
+    key, value = FusedPagedKV.read(cache, seq, pos, dtype)
+    assert value.isfinite().all()
+    out = FusedPagedDecodeAttention.apply(q, cache, torch.tensor([n], dtype=torch.int32, device=DEV), 0.125)
+    check_decode(out, q, [key], [value], [n], 0.125, 0, dtype)
+    assert out.abs().max() < 10.0
