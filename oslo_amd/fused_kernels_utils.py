@@ -25,6 +25,7 @@ import threading
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, kernels
@@ -35,10 +36,16 @@ _custom_kernels = None
 def _needs_grad(*tensors):
     """False when autograd would record nothing: the operators then call the
     kernels directly and skip the autograd.Function machinery (a decoding step
-    is bound by such per-call overheads, not by its kernels)."""
+    is bound by such per-call overheads, not by its kernels). A tangent of
+    forward-mode differentiation counts, which ``no_grad`` does not turn off: no operator
+    here computes one, and the Function machinery says so."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 return True
     return False
 
@@ -764,7 +771,7 @@ class FusedPackedAttention(object):
 
 def _refuse_grad(what, *tensors):
     if _needs_grad(*tensors):
-        raise RuntimeError(f"{what} is for inference: call it under torch.no_grad()")
+        raise RuntimeError(f"{what} is for inference: call it under torch.no_grad(), without forward-mode tangents")
 
 
 class FusedPagedKV(object):
@@ -843,7 +850,8 @@ class FusedSampling(object):
     probability; equal logits go by the lower index. A temperature of 0 takes
     the largest logit. Every setting is a number or a device tensor of one value
     per row (fp32; ``top_k`` int32). Logits of -inf are never drawn, NaN counts
-    as -inf, a row of nothing else gives token -1.
+    as -inf, a row of nothing else gives token -1. Nothing is differentiated, the
+    logarithms neither.
     """
 
     @staticmethod

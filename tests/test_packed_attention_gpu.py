@@ -308,3 +308,18 @@ def test_a_capture_is_refused_while_an_eager_graph_of_the_same_leaf_lives():
         for t, w in zip((q, k, v), want):
             assert torch.equal(t.grad, w)
             t.grad.zero_()
+
+
+def test_tangents_of_forward_mode_are_refused():
+    """The operator has no formula for them: a result without its tangent would be a wrong derivative of zero."""
+    from torch.autograd import forward_ad
+    q, k, v, g = make([20, 7], 4, 2, 64, torch.bfloat16, seed=14)
+    packed = PackedSequences([20, 7], DEV)
+    want = FusedPackedAttention.apply(q, k, v, packed, 0.1)
+    with forward_ad.dual_level():
+        for i in range(3):
+            given = [forward_ad.make_dual(x, torch.ones_like(x)) if j == i else x for j, x in enumerate((q, k, v))]
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="forward mode"):
+                    FusedPackedAttention.apply(*given, packed, 0.1)
+        assert torch.equal(FusedPackedAttention.apply(q, k, v, packed, 0.1), want)

@@ -250,6 +250,31 @@ def test_rotary_tables_live_as_long_as_what_reads_them():
     assert all(r() is None for refs in tables for r in refs)
 
 
+def test_tangents_of_forward_mode_are_not_dropped():
+    """A dual tensor needs no ``requires_grad``, and ``no_grad`` does not turn it off: torch carries the tangent on
+    through both, so an operator without one has to say so."""
+    from torch.autograd import forward_ad
+
+    from oslo_amd import FusedPagedDecodeAttention, FusedPagedKV
+    from oslo_amd.fused_kernels_utils import _needs_grad
+    x = torch.zeros((4, 2, 64), dtype=torch.bfloat16)
+    pages = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    cache = PagedKV(pages, pages.clone(), torch.zeros((4, 1), dtype=torch.int32))
+    index = torch.zeros(4, dtype=torch.int32)
+    assert not _needs_grad(x, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        assert not _needs_grad(x, None)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                assert _needs_grad(x, None, dual) and forward_ad.unpack_dual(dual * 2).tangent is not None
+                for call in (lambda: FusedPagedKV.write(cache, x, dual, index, index),
+                             lambda: FusedPagedDecodeAttention.apply(dual, cache, index)):
+                    with pytest.raises(RuntimeError, match="tangent"):
+                        call()
+    assert not _needs_grad(x)
+
+
 def test_models_refuse_what_sequences_do_not_take():
     model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
     row, packed = torch.zeros((1, 6), dtype=torch.long), PackedSequences([2, 4], "cpu")
