@@ -19,7 +19,8 @@ class PackedSequences(object):
     and shared by every layer and by the backward: it holds, on ``device``, the
     list of 128-position blocks the attention kernels take their work from
     (``blocks``: int32 [2, n, 4]; the blocks with most keys first, then those
-    with most queries left first)."""
+    with most queries left first), each token's position in its own sequence
+    (``positions``) and the sequence it belongs to (``sequence``), both int32 [total]."""
 
     def __init__(self, lengths, device):
         lengths = [int(n) for n in lengths]
@@ -31,20 +32,25 @@ class PackedSequences(object):
         if self.total >= 2 ** 31:
             raise ValueError("PackedSequences: more than 2^31 - 1 tokens")
         n = np.asarray(lengths, dtype=np.int64)
-        self._starts = np.concatenate([[0], np.cumsum(n)[:-1]]).astype(np.int64) if len(n) else n
+        starts = np.concatenate([[0], np.cumsum(n)[:-1]]).astype(np.int64) if len(n) else n
         counts = -(-n // PACKED_BLOCK)
         owner = np.repeat(np.arange(len(n)), counts)
         block = np.arange(len(owner)) - np.repeat(np.cumsum(counts) - counts, counts)
         entries = np.zeros((len(owner), 4), dtype=np.int32)
-        entries[:, 0], entries[:, 1], entries[:, 2] = self._starts[owner], n[owner], block
+        entries[:, 0], entries[:, 1], entries[:, 2] = starts[owner], n[owner], block
         keys = np.minimum((block + 1) * PACKED_BLOCK, n[owner])
         queries = n[owner] - block * PACKED_BLOCK
         order = [np.argsort(-keys, kind="stable"), np.argsort(-queries, kind="stable")]
-        self.blocks = torch.from_numpy(np.stack([entries[o] for o in order])).to(device)
+        owners = np.repeat(np.arange(len(n)), n)
+        parts = [np.stack([entries[o] for o in order]).ravel(), np.arange(self.total) - starts[owners], owners,
+                 starts + n - 1]
+        # (one copy, here: inside a capture, or on whatever stream asks first, none could be made)
+        held = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(device).split([len(p) for p in parts])
+        self.blocks = held[0].view(2, len(owner), 4)
+        self.positions, self.sequence, self._last = held[1:]
         self._queries = queries[order[1]]  # of the blocks with most queries first: how many are left
         self._shared = {}
         self.kept = {}  # what the models look up for these sequences (rotary tables), for as long as they live
-        self._positions = self._sequence = None
 
     @property
     def device(self):
@@ -76,30 +82,12 @@ class PackedSequences(object):
         parts = next(p for p in range(2, group + 1) if group % p == 0 and (work[0] / p <= max(limit, 32) or p == group))
         return int((work > max(limit, 32)).sum()), parts
 
-    def _per_token(self, values):
-        return torch.from_numpy(values.astype(np.int32)).to(self.device)
-
-    @property
-    def positions(self):
-        """int32 [total] on the device: each token's position in its own sequence."""
-        if self._positions is None:
-            n = np.asarray(self.lengths, dtype=np.int64)
-            self._positions = self._per_token(np.arange(self.total) - np.repeat(self._starts, n))
-        return self._positions
-
-    @property
-    def sequence(self):
-        """int32 [total] on the device: the sequence each token belongs to."""
-        if self._sequence is None:
-            self._sequence = self._per_token(np.repeat(np.arange(len(self.lengths)), self.lengths))
-        return self._sequence
-
     def last_tokens(self):
         """int64 [sequences] on the device: the row of each sequence's last token
         (sequences must not be empty)."""
         if any(n == 0 for n in self.lengths):
             raise ValueError("PackedSequences: an empty sequence has no last token")
-        return torch.from_numpy(self._starts + np.asarray(self.lengths, dtype=np.int64) - 1).to(self.device)
+        return self._last.to(torch.int64)
 
 
 class PagedKV(object):

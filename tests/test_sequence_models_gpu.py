@@ -383,3 +383,40 @@ def test_rotary_tables_made_inside_a_capture_are_not_handed_on():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(made[0], other[0]) and torch.equal(made[1], other[1])
+
+
+@pytest.mark.parametrize("family", FAMILIES)
+def test_a_capture_is_the_first_to_use_packed_sequences(family):
+    """Made before the capture, but used by nobody: positions, owners and last tokens of prompts that go into the cache."""
+    model, _ = make(family)
+    lengths = [37, 1, 60]
+    ids = tokens(sum(lengths), 3)[None].to(DEV)
+
+    def prompts(packed, state):
+        h = model.transformer(ids, None, state.prompt_layers(packed))[0][0]
+        return model.lm_head(h.index_select(0, packed.last_tokens()))
+
+    def fresh():
+        return (PackedSequences(lengths, DEV), PagedState(lengths, 64, len(model.transformer.h), 2,
+                                                          128 if family == "gptj" else 64, torch.float16, DEV))
+    with torch.no_grad():
+        packed, state = fresh()
+        want = prompts(packed, state)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            prompts(*fresh())
+        torch.cuda.current_stream().wait_stream(side)
+        other, caches = fresh()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = prompts(other, caches)
+        for seed in (3, 4, 5):
+            ids.copy_(tokens(sum(lengths), seed)[None])
+            graph.replay()
+            want = prompts(packed, state)
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            for a, b in zip(state.caches, caches.caches):
+                assert torch.equal(a.key_pages, b.key_pages) and torch.equal(a.value_pages, b.value_pages)

@@ -275,6 +275,21 @@ def test_tangents_of_forward_mode_are_not_dropped():
     assert not _needs_grad(x)
 
 
+def test_packed_sequences_are_whole_once_they_are_made(monkeypatch):
+    """Nothing is copied from the host later (a capture allows no such copy): positions, owners and last tokens too."""
+    packed = PackedSequences([3, 1, 4], "cpu")
+
+    def refuse(*args, **kwargs):
+        raise AssertionError("made from host data")
+    monkeypatch.setattr(torch, "from_numpy", refuse)
+    monkeypatch.setattr(torch, "tensor", refuse)
+    assert packed.positions.tolist() == [0, 1, 2, 0, 0, 1, 2, 3] and packed.sequence.tolist() == [0, 0, 0, 1, 2, 2, 2, 2]
+    last = packed.last_tokens()
+    assert last.tolist() == [2, 3, 7] and last.dtype == torch.int64
+    assert packed.blocks.is_contiguous() and packed.blocks.tolist()[0] == [[4, 4, 0, 0], [0, 3, 0, 0], [3, 1, 0, 0]]
+    assert sequence_layers(packed, 1)[0].row_positions(9).tolist() == [0, 1, 2, 0, 0, 1, 2, 3, 0]
+
+
 def test_models_refuse_what_sequences_do_not_take():
     model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
     row, packed = torch.zeros((1, 6), dtype=torch.long), PackedSequences([2, 4], "cpu")
