@@ -280,7 +280,7 @@ class GenerationMixin(object):
         def choose(scores):
             if not do_sample:
                 return scores.argmax(dim=-1)
-            uniforms = torch.rand(scores.size(0), generator=generator, device=scores.device)
+            uniforms = torch.rand(scores.size(0), generator=generator, dtype=torch.float32, device=scores.device)
             # (a row without any finite score has no token, -1: 0, which argmax gives there)
             return FusedSampling.apply(scores, uniforms, **settings)[0].clamp_(min=0)
 

@@ -206,3 +206,29 @@ def test_generate_same_tokens_before_and_after_fuse(family):
     # the switch can also come from the configuration (oslo/generation_utils.py:753-757)
     model.config.fused_no_repeat_ngram_blocking = True
     assert torch.equal(before, model.generate(ids, **kw))
+
+
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16], ids=["float64", "bfloat16"])
+def test_sampling_does_not_depend_on_the_default_dtype(default, monkeypatch):
+    """The uniform numbers are what the operator takes, whatever type tensors have by default."""
+    from oslo_amd import generation_utils
+    model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
+    seen = []
+
+    class Draw(object):
+        @staticmethod
+        def apply(logits, uniforms, **settings):
+            seen.append(uniforms)
+            return (uniforms * logits.size(-1)).long(), None
+    monkeypatch.setattr(generation_utils, "FusedSampling", Draw)
+    ids = torch.zeros((2, 3), dtype=torch.long)
+    before = torch.get_default_dtype()
+    runs = []
+    try:
+        for dtype in (before, default):
+            torch.set_default_dtype(dtype)
+            runs.append(model.generate(ids, max_length=6, do_sample=True, generator=torch.Generator().manual_seed(1)))
+    finally:
+        torch.set_default_dtype(before)
+    assert all(u.dtype == torch.float32 and u.shape == (2,) for u in seen)
+    assert torch.equal(*runs)
