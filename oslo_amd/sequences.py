@@ -201,6 +201,9 @@ class PagedState(object):
 
     def prompt_layers(self, packed):
         """``layer_past`` of every layer for the prompts, packed into one row."""
+        if len(packed.lengths) > self.table.shape[0] or packed.max_length > self.capacity:
+            raise ValueError(f"PagedState: {len(packed.lengths)} prompts of up to {packed.max_length} tokens, places for "
+                             f"{self.table.shape[0]} of up to {self.capacity}")
         shared = {}
         return [PackedLayer(packed, cache, shared) for cache in self.caches]
 

@@ -290,6 +290,16 @@ def test_packed_sequences_are_whole_once_they_are_made(monkeypatch):
     assert sequence_layers(packed, 1)[0].row_positions(9).tolist() == [0, 1, 2, 0, 0, 1, 2, 3, 0]
 
 
+def test_prompts_that_a_state_has_no_place_for_are_refused():
+    """The cache passes over tokens that name no place of it: prompts would be cut without a word."""
+    state = PagedState([4, 2], 8, 3, 1, 64, torch.float16, "cpu", page_size=16)
+    for bad in ([4, 2, 1], [9, 2], [16, 1]):
+        with pytest.raises(ValueError, match="places for 2 of up to 8"):
+            state.prompt_layers(PackedSequences(bad, "cpu"))
+    for good in ([4, 2], [8, 8], [3], []):
+        assert len(state.prompt_layers(PackedSequences(good, "cpu"))) == 3
+
+
 def test_models_refuse_what_sequences_do_not_take():
     model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
     row, packed = torch.zeros((1, 6), dtype=torch.long), PackedSequences([2, 4], "cpu")
