@@ -15,12 +15,13 @@ The bar is 1.05 times the sum for the output, twice the sum for the gradients
 (both roundings of P and dS meet in them), each with 2^-15 of the summed
 magnitudes added."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 
-from oslo_amd import FusedPackedAttention, FusedPrefillAttention, PackedSequences, kernels
+from oslo_amd import FusedPackedAttention, FusedPrefillAttention, PackedSequences, _lib, kernels
 from tests.util import IDS, randn
 
 pytestmark = pytest.mark.gpu
@@ -323,3 +324,39 @@ def test_tangents_of_forward_mode_are_refused():
                 with mode(), pytest.raises(RuntimeError, match="forward mode"):
                     FusedPackedAttention.apply(*given, packed, 0.1)
         assert torch.equal(FusedPackedAttention.apply(q, k, v, packed, 0.1), want)
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=IDS.get)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_what_the_outputs_rounding_left_out_counts(d, dtype):
+    """delta = sum dO O stands against dP in every dS of a row. Where a query sees two keys, O's own rounding is as
+    large an error in it as the others together (those of P and dS before their products, and of the gradients): the
+    formulas in 64 bits with each of these roundings applied are off by 0.0024 of dQ's and dK's norms in bf16, and by
+    0.0037 with delta from the rounded O, 1.5 times as much, at every head size and in either type. Asked for: 1.25."""
+    lengths, heads, window, scale = [260, 1, 100], 3, 2, 1.0 / math.sqrt(d)
+    q, k, v, g = make(lengths, heads, heads, d, dtype, seed=d)
+    packed = PackedSequences(lengths, DEV)
+    want, _ = reference(q, k, v, g, lengths, scale, window)
+    out, low, lse = kernels.attention_packed_forward(q, k, v, packed, scale, window, want_lse=True)
+    exact = out.double() + low.double()
+    assert (exact - want[0]).norm() < (out.double() - want[0]).norm()
+    with_low = kernels.attention_packed_backward(g, q, k, v, out, low, lse, packed, scale, window)
+    zeros = kernels.attention_packed_backward(g, q, k, v, out, torch.zeros_like(low), lse, packed, scale, window)
+    # the same through the library's own argument: no tensor
+    none = [torch.empty_like(x) for x in (q, k, v)]
+    t, blocks = q.shape[0], packed.blocks
+    lib = _lib.load()
+    size = lib.oslo_attention_packed_bwd_workspace_bytes(t, heads, heads, d, 0, 1)
+    workspace = torch.empty(size // 4, dtype=torch.float32, device=DEV)
+    strides = (ctypes.c_int64 * 16)(*([d, heads * d] * 8))
+    _lib.check(lib.oslo_attention_packed_bwd(
+        *(x.data_ptr() for x in none), g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None,
+        lse.data_ptr(), workspace.data_ptr(), blocks[0].data_ptr(), blocks[1].data_ptr(), blocks.shape[1], 0, 1, scale, t,
+        packed.max_length, heads, heads, d, window, strides, 1 if dtype == torch.float16 else 2,
+        torch.cuda.current_stream().cuda_stream))
+    for x, y in zip(none, zeros):
+        assert torch.equal(x, y)
+    for i, name in ((0, "dq"), (1, "dk")):
+        errors = [float((x[i].double() - want[1 + i]).norm()) for x in (with_low, zeros)]
+        assert errors[1] >= 1.25 * errors[0], (name, [e / float(want[1 + i].norm()) for e in errors])
+    assert torch.equal(with_low[2], zeros[2])
