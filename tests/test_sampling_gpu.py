@@ -251,3 +251,31 @@ def test_temperatures_next_to_zero():
         each = torch.full((rows,), 2.0 ** -149, device=DEV)
         check(x, u, temperature=each, top_p=0.5)
         check(x, u, temperature=2.0 ** -149, top_p=0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=IDS.get)
+@pytest.mark.parametrize("rows", [3, 257], ids=["few-rows", "many-rows"])
+def test_rows_of_as_many_logits_as_are_taken(rows, dtype):
+    """500000, and one fewer (rows then begin anywhere). Each mass is off by at most half a unit, 2^-43, so the
+    logarithm of their sum by V * 2^-43 / sum; a border of the plain code lies that close to a running sum (some 1e-7
+    of the largest mass, where a token's is 1e-3 and more on average) in one draw of ten thousand."""
+    for vocab in (500000, 499999):
+        g = torch.Generator(DEV).manual_seed(vocab)
+        logits = (torch.randn((rows, vocab), generator=g, device=DEV) * 2.5).to(dtype)
+        u = torch.rand((rows,), generator=g, device=DEV)
+        some = slice(0, 3)
+        for kw in (dict(), dict(temperature=0.6, top_k=50), dict(top_k=3000, top_p=0.9), dict(top_p=0.9), dict(min_p=0.01)):
+            tokens, logprobs = FusedSampling.apply(logits, u, **kw)
+            want, want_log = plain(logits[some], u[some], **kw)
+            assert torch.equal(tokens[some], want), kw
+            masses = torch.exp(logits[some].double() - logits[some].double().amax(1, keepdim=True)).sum(1)
+            slack = vocab * 2.0 ** -43 / (masses if not kw else torch.ones_like(masses))
+            assert ((logprobs[some].double() - want_log).abs() <= 1.1 * 2.0 ** -24 * want_log.abs() + slack).all(), kw
+            few = FusedSampling.apply(logits[-2:], u[-2:], **kw)
+            assert torch.equal(tokens[-2:], few[0]) and torch.equal(logprobs[-2:], few[1]), kw
+        logits.fill_(1.5)  # (equal masses: exact sums)
+        for kw, keep in ((dict(), vocab), (dict(top_k=4321), 4321), (dict(top_p=0.5), -(-vocab // 2)), (dict(top_k=1000), 1000)):
+            tokens = FusedSampling.apply(logits, u, **kw)[0]
+            assert torch.equal(tokens, torch.floor(u.double() * keep).long()), kw
+    with pytest.raises(RuntimeError):
+        FusedSampling.apply(torch.zeros((1, 500001), dtype=dtype, device=DEV), u[:1])
