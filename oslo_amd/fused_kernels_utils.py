@@ -697,10 +697,14 @@ def _check_captured_leaves(out):
     """A leaf's gradient is added up on the stream of the first graph that holds
     it. Captured into a HIP graph while an eager graph of that leaf lives, that
     addition would leave the capture and end the process: it is refused instead.
-    ``out``: a recorded result, whose graph holds the leaves by now."""
+    ``out``: a recorded result, whose graph holds the leaves by now. Looked at are the
+    inputs that are leaves, or made from one by operations of one input (views, copies)."""
     capturing = None
     for node, _ in out.grad_fn.next_functions:
-        if getattr(node, "variable", None) is None:  # (not a leaf)
+        while node is not None and getattr(node, "variable", None) is None:  # (not a leaf)
+            behind = node.next_functions
+            node = behind[0][0] if len(behind) == 1 else None
+        if node is None:
             continue
         if capturing is None:
             capturing = torch.cuda.is_current_stream_capturing()

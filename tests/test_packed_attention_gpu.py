@@ -360,3 +360,29 @@ def test_what_the_outputs_rounding_left_out_counts(d, dtype):
         errors = [float((x[i].double() - want[1 + i]).norm()) for x in (with_low, zeros)]
         assert errors[1] >= 1.25 * errors[0], (name, [e / float(want[1 + i].norm()) for e in errors])
     assert torch.equal(with_low[2], zeros[2])
+
+
+def test_a_capture_is_refused_while_an_eager_graph_of_the_views_leaf_lives():
+    packed = PackedSequences([40], DEV)
+    leaf = torch.randn(40, 3, 2, 64, device=DEV, dtype=torch.float16, requires_grad=True)
+    grad = torch.ones(40, 2, 64, device=DEV, dtype=torch.float16)
+    living = FusedPackedAttention.apply(*leaf.unbind(1), packed)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph):
+            FusedPackedAttention.apply(*leaf.unbind(1), packed)
+    torch.autograd.backward(living, grad)
+    want = leaf.grad.clone()
+    del living
+    leaf.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = FusedPackedAttention.apply(*leaf.unbind(1), packed)
+        torch.autograd.backward(out, grad)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(leaf.grad, want)
+        leaf.grad.zero_()

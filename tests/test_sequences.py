@@ -300,6 +300,27 @@ def test_prompts_that_a_state_has_no_place_for_are_refused():
         assert len(state.prompt_layers(PackedSequences(good, "cpu"))) == 3
 
 
+def test_leaves_behind_views_are_looked_at(monkeypatch):
+    """The slices of one leaf, as an attention's query, key and value are."""
+    from oslo_amd.fused_kernels_utils import _check_captured_leaves
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    leaf, other = (torch.ones((6, 12), requires_grad=True) for _ in range(2))
+
+    def result(x):
+        q, k, v = x.view(6, 3, 4).unbind(1)
+        return torch.stack([q, k.contiguous(), v.t().t()])
+    living = result(leaf)
+    _check_captured_leaves(living)
+    capturing[0] = True
+    with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+        _check_captured_leaves(result(leaf))
+    _check_captured_leaves(result(other))
+    _check_captured_leaves(result(leaf + other))  # (of two inputs: not followed)
+    del living
+    _check_captured_leaves(result(leaf))
+
+
 def test_models_refuse_what_sequences_do_not_take():
     model = GPT2LMHeadModel(GPT2Config(vocab_size=11, n_positions=8, n_embd=64, n_layer=1, n_head=1)).eval()
     row, packed = torch.zeros((1, 6), dtype=torch.long), PackedSequences([2, 4], "cpu")
