@@ -10,7 +10,8 @@
 // entries, the ones with most keys first, instead of a regular grid.
 //
 // Bound by the matrix cores where sequences are long: 9 prompts of 8299 tokens, 16 heads of 256
-// in bf16, 127 us for 84 Gflop, 0.65 Pflop/s, the rate of the dense kernel at that head size; 9144 tokens in
+// in bf16, 126 us for 84 Gflop, 0.67 Pflop/s. Short sequences cost that rate, in the dense kernel as here: 8 of 1024
+// tokens 0.66 (dense 0.665), 4 of 2048 0.87 (0.83), 8 of 2048 0.815 (0.80), 1 of 8192 1.10 (1.10). 9144 tokens in
 // 7 documents, 32 query heads on 8 of 128, 210 us with the statistics for the backward, 0.85 Pflop/s.
 // With a window of 256 (8794 tokens, 20 heads of 128, fp16: 73 us) the blocks walk 12 tiles of 32 keys each
 // and reading their queries and writing their outputs weighs as much as the products.

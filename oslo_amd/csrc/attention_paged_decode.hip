@@ -70,7 +70,7 @@ struct Mfma16<f16> {
   }
 };
 
-constexpr int kMinChunk = kTileKeys; // keys: one tile (300 positions x 12 heads: 8.4 us with 32, 9.4 with 64, 11.3 with 128)
+constexpr int kMinChunk = kTileKeys; // keys: one tile (by chunks, 4 sequences of 150 to 300 positions x 12 heads of 64: 8.0 us with 32, 8.6 with 64, 10.0 with 128)
 constexpr int kMaxSequences = 4096; // of one launch: the chunk list of a block lies in LDS
 
 // Chunks aimed at for `waves` waves when each of `rows` (sequences x key/value heads)
@@ -235,10 +235,11 @@ __device__ __forceinline__ int list_chunks(const PagedDecodeArgs &a, int *first,
   return chunk;
 }
 
-// Blocks of a CU the kernel is compiled (and the grid is sized) for. (Four at 128 features: 129 us
-// instead of 96 at 131071 positions; six at 64: 81 instead of 56 at 8 x 16000 positions. In 8 bits a tile
-// takes half the registers: four at 128 features, 105 us instead of 109 at 128 sequences of 100 to 8191 positions;
-// five spill, and three at 256 do: 325 instead of 191.)
+// Blocks of a CU the kernel is compiled (and the grid is sized) for. (Both launches, bf16. Four at 128 features:
+// 121 us instead of 94 at 131071 positions x 8 heads; six at 64: 59 instead of 40 at 8 sequences of 800 to 16000
+// positions x 12 heads. In 8 bits a tile takes half the registers: four at 128 features, 189 us instead of three's 194
+// at 128 sequences of 98 to 8191 positions x 8 heads, evenly spread; five spill, and three at 256 do: 351 instead of
+// 202 at 128 sequences of 102 to 2048 positions x 16 heads.)
 constexpr int blocks_per_cu(int D, bool e4m3) { return D == 256 ? 2 : D == 128 && !e4m3 ? 3 : 4; }
 
 // MEET: a block per sequence and head slot, whose waves share its tiles and meet in LDS.
@@ -634,10 +635,13 @@ __global__ __launch_bounds__(kBlockThreads) void attention_paged_join_kernel(con
 }
 
 // Where a sequence can have no more than so many tiles, a block takes it: its waves meet
-// in LDS, and one launch is all. In us, against chunks and a join, with the blocks there are:
-//   64 features x 12 heads:  1 x 300 positions 4.4 (7.4), 4 x 300 5.7 (8.0), 32 x 1024 15.2 (16.3), 400 x 1024 111 (122);
-//   128 x 8, 32 query heads: 4 x 512 7.8 (8.9), 4 x 1024 14.2 (10.5), 32 x 1024 19.6 (22.5), 32 x 2048 33 (31);
-//   256 x 16:                4 x 256 7.7 (9.8), 1 x 512 13.7 (8.8), 16 x 512 17.7 (19.2), 32 x 2048 116 (95).
+// in LDS, and one launch is all. In us, against chunks and a join in brackets, bf16, one captured call after
+// the other; n x L: n sequences of L / 2 to L positions, evenly spread (one of L), under a table of L:
+//   64 features x 12 heads:  1 x 300 5.4 (7.7), 4 x 300 5.4 (8.1), 32 x 1024 18.2 (20.1), 400 x 1024 142 (165);
+//   128 x 8, 32 query heads: 4 x 512 10.4 (9.2), 4 x 1024 17.1 (10.8), 32 x 1024 21 (25.5), 32 x 2048 37.5 (42.9);
+//   256 x 16:                4 x 256 9.8 (9.9), 1 x 512 15.1 (9.0), 16 x 512 19.3 (24.1), 32 x 2048 128 (132).
+// A fraction more could be gained: at 4 x 512 x 8 heads the rule takes the slower way, at 32 x 2048 too. A call that
+// finds its keys in no cache waits longer: 4 sequences of up to 300 positions, 12 heads of 64, 7.6 us.
 // (Asked for all sequences of a call, not for those of one of its launches: the workspace
 // has to fit every launch.)
 inline int64_t meet_tiles(int64_t blocks, int64_t head_dim) { return blocks >= 256 ? 32 : head_dim == 256 ? 8 : 16; }

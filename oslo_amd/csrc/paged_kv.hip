@@ -89,8 +89,10 @@ __device__ __forceinline__ void store_e4m3(unsigned char *pages, unsigned char *
 
 // A group of D / 8 lanes takes ROWS (token, head) rows, all loads of a thread issued
 // before any is used; ROWS is 2 where the rows fill the card four times over, else 1
-// (a decoding step: more, shorter blocks). 17206 tokens x 16 heads x 256 features,
-// 8-bit: 91, 83, 87 and 96 us with 1, 2, 4 and 8 rows (5.1 TB/s with 2).
+// (a decoding step: more, shorter blocks). One row against two, us, 8-bit: 256 tokens x 16 heads x 256 features
+// 3.5, 4.4; 2048 tokens 12.8, 11.7; 4096 (where two begins) 23.1, 21.8; 17206 89, 80 (5.3 TB/s; 4 and 8 rows
+// were slower than 2). 12 heads of 64: 256 tokens 3.2, 4.0; 17206 19.8, 20.1. In 16 bits two gain in the
+// middle, 2048 tokens x 16 x 256 12.3, 10.6, and cost some at the end, 17206 tokens 86, 91.
 template <typename T, int D, bool E4M3, int ROWS>
 __global__ __launch_bounds__(kBlockThreads) void paged_kv_write_kernel(const PagedKVArgs a) {
   constexpr int kLanes = D / 8;
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(kBlockThreads) void paged_kv_write_kernel(const Pag
   }
 }
 
-// One row per group of lanes: 77, 80, 85 and 97 us with 1, 2, 4 and 8 for the same tokens
+// One row per group of lanes: 77, 80, 85 and 97 us with 1, 2, 4 and 8 for 17206 tokens x 16 x 256, 8-bit
 // (5.5 TB/s with 1).
 template <typename T, int D, bool E4M3>
 __global__ __launch_bounds__(kBlockThreads) void paged_kv_read_kernel(const PagedKVArgs a) {

@@ -19,7 +19,7 @@
 //
 // One block takes a row, 1024 threads and a CU for itself up to 256 rows; beyond that
 // 512, two to a CU, one waiting for memory or at a barrier while the other computes
-// (1000 rows of 50257 fp32 logits with top-p: 127 against 155 us when this was chosen, 120 now). It holds the row in
+// (1000 rows of 50257 fp32 logits with top-p: 118 against 130 us). It holds the row in
 // registers and LDS (53248 logits of 32 bits, or 20480, twice that in 16 bits; what exceeds them
 // is read again, ahead of its use), each wave a run of it. Such a row is read in 5 to 8 us; what
 // costs the time then is arithmetic, one operation in 64 bits after another, and
@@ -40,7 +40,10 @@
 //    chunk, which all waves sum together, and looks inside that.
 // Windows too full for the list (equal logits by the thousand) are searched by
 // histograms over the bits of the logits. Measured, us a call: one row of 50257 fp32 logits, top-k 50 and
-// top-p, 12.3; 256 rows in bf16, settings of their own, 36; 1000 rows in fp32, top-p 0.92, 118 to 127.
+// top-p, 12.1; 256 rows in bf16, settings of their own, 35; 1000 rows in fp32, top-p 0.92, 118 captured, 125 eager, 132
+// under the profiler, which counts 475 MB read, 2.4 times the logits: what a row has beyond the 20480 that are held comes
+// again for the maximum, the count and the exact pass, at 3.8 TB/s on average next to some sixty vector
+// instructions a logit, many of them in 64 bits.
 
 #include "common.hpp"
 
@@ -1001,8 +1004,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(const SampleArgs a)
 
 // Logits a row may have: its chunks have to fit the bins, and the list.
 constexpr int64_t kMaxVocab = 500000;
-// A block of 1024 threads per row while every row gets a CU of its own (256 rows with top-p: 40 us); smaller
-// blocks gain only where two share a CU (1000 rows: 127 against 155 us).
+// A block of 1024 threads per row while every row gets a CU of its own; smaller blocks gain where two share a CU. In us,
+// 512 threads against 1024, 50257 logits, top-p 0.92: 256 rows 46 against 37 in fp32, 39 against 34 in bf16; 257 rows 56
+// against 62, 53 against 62; 512 rows 65 against 69, 58 against 67; 1000 rows 118 against 130, 106 against 130. (With top-k 50:
+// 256 rows 23 against 18, 257 24 against 28, 768 50 against 50 in fp32; without filters 31, 25, 40, 42, 66, 69.)
 constexpr int64_t kRowsAtOnce = 256;
 static_assert(kMaxVocab + 8 <= (int64_t)kBins * kWave * 4 - kMostWaves * kWave * 4, "a bin per chunk");
 
