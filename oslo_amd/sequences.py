@@ -41,11 +41,12 @@ class PackedSequences(object):
         keys = np.minimum((block + 1) * PACKED_BLOCK, n[owner])
         queries = n[owner] - block * PACKED_BLOCK
         order = [np.argsort(-keys, kind="stable"), np.argsort(-queries, kind="stable")]
-        owners = np.repeat(np.arange(len(n)), n)
-        parts = [np.stack([entries[o] for o in order]).ravel(), np.arange(self.total) - starts[owners], owners,
-                 starts + n - 1]
+        positions = np.arange(self.total, dtype=np.int32)
+        positions -= np.repeat(starts.astype(np.int32), n)
+        parts = [entries[np.concatenate(order)].ravel(), positions, np.repeat(np.arange(len(n), dtype=np.int32), n),
+                 (starts + n - 1).astype(np.int32)]
         # (one copy, here: inside a capture, or on whatever stream asks first, none could be made)
-        held = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(device).split([len(p) for p in parts])
+        held = torch.from_numpy(np.concatenate(parts)).to(device).split([len(p) for p in parts])
         self.blocks = held[0].view(2, len(owner), 4)
         self.positions, self.sequence, self._last = held[1:]
         self._queries = queries[order[1]]  # of the blocks with most queries first: how many are left
