@@ -12,7 +12,7 @@ timed region. The JSON line printed at the end carries
   roofline      the causal forward kernel alone (its launches timed with events
                 on the launch stream), as a fraction of the 8 TB/s HBM peak
   kernels       the same figure for every other kernel of the path at its
-                benchmark shape
+                benchmark shape (short rows; all columns on the error stream)
   cpu_baseline  the reference's unfused arithmetic on the host cores, timed on
                 a bounded sample of the same workload
 
@@ -243,15 +243,26 @@ def main():
     if not args.no_cpu_baseline:
         out["cpu_baseline"] = cpu_baseline(torch, section)
     # The figures a reader of the first kilobytes of the line needs, inside `config`: the second half
-    # of the metric (GPT-J-shaped forward, tokens/s, unfused against fuse()), the training step, and
-    # the fraction of its roofline of every kernel of the table.
+    # of the metric (GPT-J-shaped forward, tokens/s, unfused against fuse()) and the training step.
     for key in ("gptj_fwd", "gptj_train_step"):
         sec = out.get(key)
         if isinstance(sec, dict):
             out["config"][key] = {k: sec[k] for k in ("unfused_tokens_per_s", "fused_tokens_per_s", "speedup",
                                                       "logits_vs_fp32", "error") if k in sec}
-    out["config"]["kernel_fracs"] = {k["kernel"]: k["frac"] for k in kernels}
-    print(json.dumps(out))
+    print(json.dumps({"kernels": kernels}), file=sys.stderr)
+    print(short_line(out))
+
+
+SHORT_ROW = ("kernel", "us", "achieved", "frac", "traffic")
+
+
+def short_line(out):
+    """The record as one line that is kept whole where output is cut at some
+    kilobytes (it had grown past 20000 characters): of a kernel row its name, time,
+    rate (GB/s; TFLOP/s of the matrix products), fraction of the peak and
+    measured bytes; the rows with all they hold go to the error stream."""
+    rows = [{key: row[key] for key in SHORT_ROW if row.get(key) is not None} for row in out["kernels"]]
+    return json.dumps({**out, "kernels": rows})
 
 
 def other_kernels(lib, torch, dev, st, P, check, time_launches, roof, n):
