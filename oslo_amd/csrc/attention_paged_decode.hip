@@ -50,6 +50,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // The reference maximum of a query follows the scores when one exceeds it by more
 // than this (log2 units): exponentials up to 2^8 are as exact as those up to 1.
 constexpr float kRise = 8.0f;
+constexpr float kLeastScore = -3.40282347e38f; // the lowest finite number
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -473,8 +474,9 @@ __global__ __launch_bounds__(kBlockThreads, blocks_per_cu(D, E4M3)) void attenti
       // some query's reference rises (or this is the wave's first tile)
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      const float m_new = fmaxf(m, top);
-      const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+      // (a finite one: keys whose scores are all -inf count as nothing, until one has a score)
+      const float m_new = fmaxf(fmaxf(m, top), kLeastScore);
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new); // (0 in the first tile, where nothing is summed)
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < kBlocksD; ++i) o[i] *= alpha;

@@ -432,3 +432,26 @@ def test_large_values_of_keys_that_do_not_count(d):
     out = FusedPagedDecodeAttention.apply(q, cache, torch.tensor([n], dtype=torch.int32, device=DEV), 0.125)
     check_decode(out, q, [key], [value], [n], 0.125, 0, dtype)
     assert out.abs().max() < 10.0
+
+
+@pytest.mark.parametrize("n,heads,kv_heads,d", [(70, 4, 2, 64), (300, 2, 2, 128), (900, 16, 1, 256), (6000, 4, 4, 64)],
+                         ids=lambda v: str(v))
+def test_keys_with_infinite_scores_count_as_nothing(n, heads, kv_heads, d):
+    """Scores of -inf, over whole tiles and chunks, at the start, in the middle and at the end, beside ordinary ones;
+    only such scores: NaN, as the formula gives."""
+    dtype = torch.bfloat16
+    cache = poisoned([n, n], kv_heads, d, 64, dtype, False)
+    seq, pos = tokens_of([n, n])
+    k, v = (randn((2 * n, kv_heads, d), dtype, seed=s).to(DEV) for s in (1, 2))
+    q = randn((2, heads, d), dtype, seed=3).to(DEV)
+    q[..., 0] = 1.0
+    at = torch.arange(n, device=DEV)
+    gone = (at < n // 3) | ((at > n // 2) & (at < n // 2 + 5)) | (at >= n - 40)
+    k[:n][gone, :, 0] = -math.inf
+    k[n:, :, 0] = -math.inf
+    FusedPagedKV.write(cache, k, v, seq, pos)
+    out = FusedPagedDecodeAttention.apply(q, cache, torch.tensor([n, n], dtype=torch.int32, device=DEV), 0.1)
+    check_decode(out[:1], q[:1], [k[:n]], [v[:n]], [n], 0.1, 0, dtype)
+    assert out[1].isnan().all()
+    rest = FusedPagedDecodeAttention.apply(q, cache, torch.tensor([n // 3 + 1, n], dtype=torch.int32, device=DEV), 0.1, 1)
+    assert torch.equal(rest[0], v[n // 3].repeat_interleave(heads // kv_heads, 0))
