@@ -553,7 +553,8 @@ __global__ __launch_bounds__(kBlockThreads, D == 256 ? 1 : D == 128 ? 2 : 3) voi
             // wave: its reference then is a floor so far down that the first
             // visible score overflows the tile's sum, which has the tile done
             // again in plain order, where the reference rises to that score.
-            m = HAS_WINDOW ? fmaxf(mt, kReferenceFloor) : mt;
+            // (The same where the first keys of a packed sequence score -inf.)
+            m = HAS_WINDOW || PACKED ? fmaxf(mt, kReferenceFloor) : mt;
           }
         }
 #pragma unroll

@@ -386,3 +386,25 @@ def test_a_capture_is_refused_while_an_eager_graph_of_the_views_leaf_lives():
         torch.cuda.synchronize()
         assert torch.equal(leaf.grad, want)
         leaf.grad.zero_()
+
+
+@pytest.mark.parametrize("window", [0, 150])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_keys_with_infinite_scores_count_as_nothing(d, window):
+    """Scores of -inf over whole tiles at a sequence's start and later, beside ordinary ones; a query that sees no other:
+    NaN, as the formula gives."""
+    lengths, dtype, scale = [300, 5, 170], torch.bfloat16, 0.1
+    q, k, v, _ = make(lengths, 4, 2, d, dtype, seed=d + window)
+    packed = PackedSequences(lengths, DEV)
+    q[..., 0] = 1.0
+    at = torch.cat([torch.arange(n, device=DEV) for n in lengths])
+    gone = (at < 70) | ((at > 100) & (at < 103)) | ((at > 128) & (at < 200))
+    gone[300:305] = False
+    k[gone, :, 0] = -math.inf
+    out = FusedPackedAttention.apply(q, k, v, packed, scale, window or None)
+    trained = FusedPackedAttention.apply(q.clone().requires_grad_(True), k, v, packed, scale, window or None)
+    want, mag = reference(q, k, v, torch.zeros_like(q), lengths, scale, window)
+    sees = ~want[0].isnan().any(-1).any(-1)
+    assert sees.sum() == 475 - 140 and out[~sees].isnan().all()
+    check(out[sees], want[0][sees], mag[0][sees], dtype, 1.05, "out")
+    assert torch.equal(trained[sees], out[sees])
